@@ -75,12 +75,19 @@ _SIGS = {
     "ggs_upfirdn2d_t": (C.c_int, [C.c_int] * 5 + [_PTR, _PTR] + [C.c_int] * 10 + [_PTR, _PTR]),
     "ggs_upfirdn2d_out_size": (C.c_int, [C.c_int] * 12 + [C.POINTER(C.c_int), C.POINTER(C.c_int)]),
     "ggs_upfirdn2d": (C.c_int, [C.c_int] * 4 + [_PTR, _PTR] + [C.c_int] * 10 + [_PTR, _PTR]),
+    "ggs_rms_norm_forward": (C.c_int, [C.c_int, C.c_size_t, C.c_int, C.c_size_t] + [_PTR] * 3 + [C.c_int, C.c_double] + [_PTR] * 4),
+    "ggs_rms_norm_workspace_bytes": (C.c_size_t, [C.c_int, C.c_size_t, C.c_int, C.c_size_t]),
+    "ggs_rms_norm_backward": (C.c_int, [C.c_int, C.c_size_t, C.c_int, C.c_size_t] + [_PTR] * 3 + [C.c_int] + [_PTR] * 6 + [C.c_size_t, _PTR]),
     "ggs_adam_state_bytes": (C.c_size_t, []),
     "ggs_adam_tick": (C.c_int, [_PTR, C.c_double, C.c_double, _PTR, _PTR]),
     "ggs_adam_step": (C.c_int, [C.c_size_t, _PTR, _PTR, _PTR, _PTR, _PTR, C.c_double, C.c_double, C.c_double, _PTR, _PTR, _PTR]),
     "ggs_adam_tick_multi": (C.c_int, [C.c_int, _PTR, C.c_double, C.c_double, _PTR, _PTR]),
     "ggs_adam_step_multi": (C.c_int, [C.c_int] + [_PTR] * 7 + [C.c_double] * 3 + [_PTR] * 2),
     "ggs_adam_tick_step_multi": (C.c_int, [C.c_int] + [_PTR] * 7 + [C.c_double] * 3 + [_PTR] * 2),
+    "ggs_grad_norm_workspace_bytes": (C.c_size_t, [C.c_int]),
+    "ggs_grad_norm": (C.c_int, [C.c_int] + [_PTR] * 5 + [C.c_size_t, _PTR]),
+    "ggs_grad_clip": (C.c_int, [C.c_int] + [_PTR] * 3 + [C.c_double] + [_PTR] * 2 + [C.c_size_t, _PTR]),
+    "ggs_adam_clip_step": (C.c_int, [C.c_int] + [_PTR] * 7 + [C.c_double] * 4 + [C.c_int] + [_PTR] * 3 + [C.c_size_t, _PTR]),
     "ggs_registration_aux": (C.c_int, [C.c_int] + [_PTR] * 7 + [C.c_float] * 4 + [_PTR] * 9),
     "ggs_registration_aux_tail": (C.c_int, [C.c_int] + [_PTR] * 7 + [C.c_float] * 4 + [_PTR] * 8 + [C.POINTER(GgsStepTail), _PTR]),
     "ggs_step_prologue": (C.c_int, [C.POINTER(GgsStepPrologue), _PTR]),
@@ -148,6 +155,23 @@ def stream_ptr(dev) -> int:
     return torch.cuda.current_stream(dev).cuda_stream
 
 
+class on_device:
+    """Makes a tensor's device the current one for the launches inside (a launch onto another device's stream is an error)."""
+
+    def __init__(self, dev):
+        self.dev = dev
+
+    def __enter__(self):
+        now = torch.cuda.current_device()
+        self.back = None if self.dev.index in (None, now) else now
+        if self.back is not None:
+            torch.cuda.set_device(self.dev)
+
+    def __exit__(self, *_):
+        if self.back is not None:
+            torch.cuda.set_device(self.back)
+
+
 def host_mapped_pointer(t) -> int:
     """Device address of a pinned host tensor (0 when the memory is not mapped into the device's address space)."""
     out = C.c_void_p()
@@ -157,7 +181,7 @@ def host_mapped_pointer(t) -> int:
 
 
 _SRC_ORDER = ("ggs_pergauss.hip", "ggs_binning.hip", "ggs_render.hip", "ggs_mesh.hip", "ggs_loss.hip", "ggs_knn.hip",
-              "ggs_stylegan.hip", "ggs_visibility.hip", "ggs_adam.hip", "ggs_regaux.hip", "ggs_api.hip", "ggs_common.h",
+              "ggs_stylegan.hip", "ggs_rmsnorm.hip", "ggs_visibility.hip", "ggs_adam.hip", "ggs_gradnorm.hip", "ggs_regaux.hip", "ggs_api.hip", "ggs_common.h",
               "ggs_kernels.h", "ggs_render_common.h", os.path.join("..", "..", "include", "ggsplat.h"), "Makefile")
 
 
@@ -202,3 +226,14 @@ def dtype_code(dt) -> int:
         return {torch.float32: 0, torch.float16: 1, torch.float64: 2}[dt]
     except KeyError:
         raise RuntimeError(f'"ggsplat stylegan op" not implemented for \'{str(dt).replace("torch.", "")}\'') from None
+
+
+_NORM_DTYPES = {torch.float32: 0, torch.float16: 1, torch.float64: 2, torch.bfloat16: 3}
+
+
+def norm_dtype_code(dt, allowed=tuple(_NORM_DTYPES)) -> int:
+    """GGS_DTYPE_* for the entry points that also take bfloat16 (ggs_rms_norm_*, ggs_grad_*)."""
+    if dt not in allowed:
+        raise TypeError(f"ggsplat: {str(dt).replace('torch.', '')} is not one of "
+                        + ", ".join(str(d).replace("torch.", "") for d in allowed))
+    return _NORM_DTYPES[dt]

@@ -8,16 +8,135 @@ optimisation step can be replayed as one hipGraph:
     `param_groups[i]["lr"]` after a schedule update -- a 4-byte-per-group async copy, no re-capture);
   * moments are allocated up front (nothing is allocated or zero-filled inside a captured step);
   * `step(guard=...)`: a device int64/uint64 word that voids the whole step when non-zero -- the binning-overflow
-    flag of the forward of the same step (ggsplat.rasterizer.last_header()[1:2]).
+    flag of the forward of the same step (ggsplat.rasterizer.last_header()[1:2]);
+  * `max_norm=...`: the update reads the gradients scaled by min(1, max_norm / (N + 1e-6)), N the norm of all gradients of the
+    step as one vector -- torch.nn.utils.clip_grad_norm_ without its pass that rewrites them and without a host sync.
+
+`grad_norm` / `clip_grad_norm_` are the same norm and scaling on any list of gradients (of another optimiser, of a bucket that
+was just all-reduced); they take GRADIENTS, like ggsplat.dist.all_reduce_grads, not parameters.
 """
 from __future__ import annotations
 
 import ctypes as C
+import math
 from typing import Dict, Iterable, List, Optional
 
 import torch
 
-from ._lib import check, lib, ptr, stream_ptr
+from ._lib import check, lib, norm_dtype_code, on_device, ptr, stream_ptr
+
+_GRAD_TYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _checked_max_norm(max_norm) -> float:
+    m = float(max_norm)
+    if not m >= 0.0:                       # NaN too
+        raise ValueError(f"ggsplat: max_norm must be a number that is not negative, got {max_norm}")
+    return m
+
+
+def _span(t: torch.Tensor):
+    """(elements from the first to the last one, whether they fill that span without gaps, whether some of them share memory)."""
+    span, dense, shared = 1, True, False
+    for stride, size in sorted(zip(t.stride(), t.size())):
+        if size > 1:
+            shared = shared or stride < span
+            dense = dense and stride == span
+            span += stride * (size - 1)
+    return span, dense, shared
+
+
+class _GradList:
+    """The gradients of one call as the C ABI takes them: sizes, addresses, types.  The order of a tensor's elements is of no
+    matter to the norm, so any dense layout is read in place; a strided one is read (and written back) through a copy."""
+
+    def __init__(self, grads, in_place: bool):
+        grads = [grads] if isinstance(grads, torch.Tensor) else [g for g in grads if g is not None]
+        self.device, self.copies, spans, kept = None, [], [], []
+        for g in grads:
+            if not isinstance(g, torch.Tensor):
+                raise TypeError(f"ggsplat: gradients are tensors, got {type(g).__name__}")
+            if g.device.type != "cuda":
+                raise RuntimeError("ggsplat: gradient norms run on the GPU only (no CPU path in the product)")
+            if g.requires_grad:
+                raise ValueError("ggsplat: pass the gradients ([p.grad for p in params]), not the parameters")
+            if g.layout != torch.strided:
+                raise TypeError("ggsplat: sparse gradients are not supported")
+            if self.device is None:
+                self.device = g.device
+            elif g.device != self.device:
+                raise ValueError("ggsplat: the gradients are on different devices")
+            code = norm_dtype_code(g.dtype, _GRAD_TYPES)
+            n = g.numel()
+            if n == 0:
+                continue
+            span, dense, shared = (n, True, False) if g.is_contiguous() else _span(g)
+            if in_place:
+                if shared:
+                    raise ValueError("ggsplat: a gradient's elements share memory (an expanded tensor?): make it contiguous first")
+                at = g.data_ptr()
+                spans.append((at, at + span * g.element_size()))
+            if not dense:
+                c = g.contiguous()
+                self.copies.append((g, c))
+                g = c
+            kept.append((n, g.data_ptr(), code, g))
+        if in_place:
+            spans.sort()
+            if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+                raise ValueError("ggsplat: two of the gradients overlap in memory (the same one listed twice?)")
+        self.n = n = len(kept)
+        self.keep = [k[3] for k in kept]
+        self.numel = (C.c_size_t * n)(*[k[0] for k in kept])
+        self.ptrs = (C.c_void_p * n)(*[k[1] for k in kept])
+        self.types = (C.c_int * n)(*[k[2] for k in kept])
+
+    def buffers(self):
+        """(the norm, workspace bytes, workspace): new for every call, so that calls on several streams and captured graphs
+        never share them."""
+        nb = int(lib().ggs_grad_norm_workspace_bytes(self.n))
+        return (torch.empty((), dtype=torch.float32, device=self.device), nb,
+                torch.empty(nb, dtype=torch.uint8, device=self.device) if nb else None)
+
+
+@torch.no_grad()
+def grad_norm(grads) -> torch.Tensor:
+    """The length of `grads` (a tensor, or tensors of float32 / float16 / bfloat16 in any mixture; None entries are skipped) as
+    ONE vector: sqrt(sum of all squares), a 0-dim float32 tensor on their device, 0 for no gradients at all.  Asynchronous on the
+    current stream, capturable; sums in double, the same bits on every run."""
+    gl = _GradList(grads, False)
+    if gl.device is None:
+        return torch.tensor(0.0)
+    with on_device(gl.device):
+        norm, nb, ws = gl.buffers()
+        check(lib().ggs_grad_norm(gl.n, gl.numel, gl.ptrs, gl.types, norm.data_ptr(), ptr(ws), nb, stream_ptr(gl.device)),
+              "ggs_grad_norm")
+    return norm
+
+
+@torch.no_grad()
+def clip_grad_norm_(grads, max_norm: float, error_if_nonfinite: bool = False) -> torch.Tensor:
+    """Scales every gradient in place by min(1, max_norm / (N + 1e-6)) and returns N = grad_norm(grads), as
+    torch.nn.utils.clip_grad_norm_ does for the gradients of its parameters (norm_type 2).  A NaN norm makes every gradient NaN,
+    an infinite one zero (NaN where it was infinite); `error_if_nonfinite` raises instead and leaves the gradients as they were,
+    which needs the norm on the host: a synchronisation, refused inside a capture.  No two gradients may overlap in memory."""
+    max_norm = _checked_max_norm(max_norm)
+    gl = _GradList(grads, True)
+    if gl.device is None:
+        return torch.tensor(0.0)
+    if error_if_nonfinite:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("ggsplat: error_if_nonfinite needs the norm on the host and cannot be captured")
+        total = float(grad_norm(gl.keep))
+        if not math.isfinite(total):
+            raise RuntimeError(f"ggsplat: the gradient norm is {total}: the gradients were not clipped")
+    with on_device(gl.device):
+        norm, nb, ws = gl.buffers()
+        check(lib().ggs_grad_clip(gl.n, gl.numel, gl.ptrs, gl.types, max_norm, norm.data_ptr(), ptr(ws), nb,
+                                  stream_ptr(gl.device)), "ggs_grad_clip")
+        for g, c in gl.copies:
+            g.copy_(c)
+    return norm
 
 
 class _LrStaging:
@@ -49,7 +168,11 @@ class _LrStaging:
 
 
 class GraphAdam:
-    def __init__(self, params: Iterable, lr: float = 0.0, betas=(0.9, 0.999), eps: float = 1e-15):
+    def __init__(self, params: Iterable, lr: float = 0.0, betas=(0.9, 0.999), eps: float = 1e-15,
+                 max_norm: Optional[float] = None):
+        """max_norm: clip the gradients of every step() by their global norm (None: no clipping).  A plain attribute that
+        step() reads: a captured step keeps the value it was captured with.  `last_grad_norm` (0-dim, on the device) is the
+        norm of the last step that was not void, before clipping."""
         groups = list(params)
         if groups and not isinstance(groups[0], dict):
             groups = [{"params": groups}]
@@ -64,6 +187,8 @@ class GraphAdam:
         if first.device.type != "cuda":
             raise RuntimeError("ggsplat GraphAdam runs on the GPU only (no CPU path in the product)")
         dev = self.device = first.device
+        self.max_norm = None if max_norm is None else _checked_max_norm(max_norm)
+        self.last_grad_norm = torch.zeros((), dtype=torch.float32, device=dev)
         L = lib()
         self._state_bytes = int(L.ggs_adam_state_bytes())
         self._lr_dev = torch.zeros(len(self.param_groups), dtype=torch.float32, device=dev)
@@ -171,6 +296,9 @@ class GraphAdam:
                 st = self.state[p]
                 items.append((p.numel(), p.data_ptr(), grad.data_ptr(), st["exp_avg"].data_ptr(),
                               st["exp_avg_sq"].data_ptr(), self._lr_dev.data_ptr() + 4 * i, st["state"].data_ptr(), grad))
+        if self.max_norm is not None:
+            self._clipped_step(L, items, tick, gp, stream)
+            return
         for k in range(0, len(items), 16):
             chunk = items[k:k + 16]
             n = len(chunk)
@@ -180,3 +308,14 @@ class GraphAdam:
             fn = L.ggs_adam_tick_step_multi if tick else L.ggs_adam_step_multi
             check(fn(n, numel, cols[0], cols[1], cols[2], cols[3], cols[4], cols[5], b1, b2, self.eps, gp, stream),
                   "ggs_adam_tick_step_multi" if tick else "ggs_adam_step_multi")
+
+    def _clipped_step(self, L, items, tick: bool, gp, stream) -> None:
+        n = len(items)
+        numel = (C.c_size_t * n)(*[c[0] for c in items])
+        cols = [(C.c_void_p * n)(*[c[j] for c in items]) for j in range(1, 7)]
+        with on_device(self.device):
+            # the partial sums of this step: allocated per step, so that two captured steps never share them
+            nb = int(L.ggs_grad_norm_workspace_bytes(n))
+            ws = torch.empty(nb, dtype=torch.uint8, device=self.device) if nb else None
+            check(L.ggs_adam_clip_step(n, numel, *cols, self.betas[0], self.betas[1], self.eps, _checked_max_norm(self.max_norm),
+                                       int(tick), gp, self.last_grad_norm.data_ptr(), ptr(ws), nb, stream), "ggs_adam_clip_step")

@@ -281,11 +281,15 @@ class MeshGaussianModel(DensifyMixin):
         # ONE launch for all seven tensors instead of ~8 foreach kernels per group (0.48 ms of host time per eager iteration,
         # 0.14 ms with torch's own fused=True: profiles/r04_host_profile.md), graph-capturable, results within 2e-6 of
         # torch.optim.Adam (tests/test_gpu_graph_step.py).  optimizer="torch" keeps the PyTorch class.
+        # training_args.max_grad_norm (absent or None: no clipping, as in the reference): GraphAdam clips by the global norm.
+        max_norm = getattr(training_args, "max_grad_norm", None)
         if optimizer == "torch" or not self._xyz.is_cuda:
+            if max_norm is not None:
+                raise ValueError("training_setup: max_grad_norm needs the GraphAdam optimiser (parameters on the GPU)")
             self.optimizer = torch.optim.Adam(groups, lr=0.0, eps=1e-15)
         else:
             from .adam import GraphAdam
-            self.optimizer = GraphAdam(groups, lr=0.0, eps=1e-15)
+            self.optimizer = GraphAdam(groups, lr=0.0, eps=1e-15, max_norm=max_norm)
         from .schedule import get_expon_lr_func
         self.xyz_scheduler_args = get_expon_lr_func(
             lr_init=pos_lr, lr_final=getattr(training_args, "position_lr_final", 0.0000016) * self.spatial_lr_scale,

@@ -35,6 +35,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from ._lib import check, lib, norm_dtype_code, on_device, ptr, stream_ptr
+
 CHANNELS = {4: 512, 8: 512, 16: 512, 32: 512, 64: 512, 128: 256, 256: 128, 512: 64, 1024: 32, 2048: 16}
 
 
@@ -149,6 +151,123 @@ def resample2d(x, k, up: int = 1, down: int = 1, pad: Tuple[int, int] = (0, 0), 
 
 
 # ------------------------------------------------------------------------------------------------------------------
+# op 3: root-mean-square norm over the channels ("pixel norm") with the residual's addition
+#   h = x + residual,  q = (mean_c h^2 + eps)^-1/2,  y = weight q h;   with n = q h:
+#   dL/dh = q (weight gy - n mean_c(weight gy n)) + gh = dL/dx = dL/dresidual,   dL/dweight = sum over pixels of gy n
+# ------------------------------------------------------------------------------------------------------------------
+_RMS_TYPES = (torch.float32, torch.float16, torch.bfloat16, torch.float64)
+
+
+def _rms_layout(x):
+    """(x as the kernels read it, outer, inner, how to bring another tensor of its shape to the same order): channels-last
+    maps and anything else whose channels are innermost are rows, the rest is [B][C][pixels]."""
+    b, c = x.shape[0], x.shape[1]
+    pixels = 1
+    for s in x.shape[2:]:
+        pixels *= s
+    if x.is_contiguous():
+        return x, (b, pixels), lambda t: t.contiguous()
+    if x.movedim(1, -1).is_contiguous():
+        return x, (b * pixels, 1), lambda t: t if t.movedim(1, -1).is_contiguous() else t.movedim(1, -1).contiguous().movedim(-1, 1)
+    return x.contiguous(), (b, pixels), lambda t: t.contiguous()
+
+
+def _rms_forward(x, weight, residual, eps, store):
+    """(y, h or None, q or None, x and residual in the kernels' order, layout)."""
+    x, (outer, inner), order = _rms_layout(x)
+    y = torch.empty_like(x)
+    h = q = None
+    if residual is not None:
+        residual = order(residual)
+        h = torch.empty_like(x)
+    if store:
+        q = torch.empty(outer * inner, device=x.device, dtype=torch.float64 if x.dtype is torch.float64 else torch.float32)
+    w = None if weight is None else weight.contiguous()
+    with on_device(x.device):
+        check(lib().ggs_rms_norm_forward(norm_dtype_code(x.dtype), outer, x.shape[1], inner, x.data_ptr(),
+                                         None if residual is None else residual.data_ptr(), ptr(w),
+                                         int(w is not None and w.dtype is torch.float32), eps, y.data_ptr(),
+                                         None if h is None else h.data_ptr(), ptr(q), stream_ptr(x.device)), "ggs_rms_norm_forward")
+    return y, h, q, x, residual, w
+
+
+class _RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        y, h, q, x, residual, w = _rms_forward(x, weight, residual, eps, True)
+        ctx.set_materialize_grads(False)
+        # float and double keep the sum; 16 bits keep both summands, because h is stored rounded (csrc/ggs_rmsnorm.hip)
+        if residual is not None and x.dtype in (torch.float32, torch.float64):
+            ctx.save_for_backward(h, None, w, q)
+        else:
+            ctx.save_for_backward(x, residual, w, q)
+        return y if residual is None else (y, h)
+
+    @staticmethod
+    def backward(ctx, gy, gh=None):
+        if torch.is_grad_enabled():                                   # create_graph=True
+            raise RuntimeError("rms_norm: its gradients are not differentiable again (create_graph=True)")
+        x, residual, w, q = ctx.saved_tensors
+        if gy is None:                                                # only h was used further on
+            return gh, None, gh if ctx.needs_input_grad[2] else None, None
+        x, (outer, inner), order = _rms_layout(x)
+        gy, gh = order(gy), None if gh is None else order(gh)
+        dx = torch.empty_like(x)
+        L, code, dw, ws, nb = lib(), norm_dtype_code(x.dtype), None, None, 0
+        with on_device(x.device):
+            if ctx.needs_input_grad[1]:
+                dw = torch.empty_like(w)
+                nb = int(L.ggs_rms_norm_workspace_bytes(code, outer, x.shape[1], inner))
+                ws = torch.empty(nb, dtype=torch.uint8, device=x.device)
+                if x.numel() == 0:
+                    dw.zero_()
+            check(L.ggs_rms_norm_backward(code, outer, x.shape[1], inner, x.data_ptr(),
+                                          None if residual is None else residual.data_ptr(), ptr(w),
+                                          int(w is not None and w.dtype is torch.float32), ptr(q), gy.data_ptr(),
+                                          None if gh is None else gh.data_ptr(), dx.data_ptr(), ptr(dw), ptr(ws), nb,
+                                          stream_ptr(x.device)), "ggs_rms_norm_backward")
+        return dx, dw, dx if ctx.needs_input_grad[2] else None, None
+
+
+def rms_norm(x, weight=None, residual=None, eps: float = 1e-8, impl: str = "hip"):
+    """y = weight[channel] * h / sqrt(mean over the channels of h^2 + eps), h = x (+ residual), for x [B, C, ...] (every pixel of a
+    feature map by itself; [rows, C]: every row).  Returns y, or (y, h) with a residual -- h is the sum to carry on.
+    x, residual: float32 / float16 / bfloat16 / float64, the same shape; weight [C]: x's type or float32; contiguous and
+    channels-last maps are taken as they are.  The norm is that of the unrounded sum; sums are in float (double for float64).
+    Differentiable once (its gradients are not differentiable again)."""
+    if x.ndim < 2 or x.shape[1] == 0:
+        raise ValueError(f"rms_norm: x must be [B, C, ...] with C > 0, got {tuple(x.shape)}")
+    if x.dtype not in _RMS_TYPES:
+        raise TypeError(f"rms_norm: {x.dtype} is not float32, float16, bfloat16 or float64")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
+        raise ValueError("rms_norm: residual must have x's shape, type and device")
+    if weight is not None and (weight.shape != (x.shape[1],) or weight.dtype not in (x.dtype, torch.float32) or weight.device != x.device):
+        raise ValueError("rms_norm: weight must be [C], of x's type or float32, on x's device")
+    eps = float(eps)
+    if not (eps > 0.0 and math.isfinite(eps)):
+        raise ValueError("rms_norm: eps must be positive")
+    if impl == "native":
+        return _rms_norm_native(x, weight, residual, eps)
+    if not x.is_cuda:
+        raise RuntimeError("rms_norm: input must be a CUDA tensor")
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (residual is not None and residual.requires_grad)):
+        return _RmsNorm.apply(x, weight, residual, eps)
+    y, h = _rms_forward(x, weight, residual, eps, False)[:2]
+    return y if residual is None else (y, h)
+
+
+def _rms_norm_native(x, weight, residual, eps):
+    """The same operator in plain PyTorch ops."""
+    wide = x.dtype if x.dtype is torch.float64 else torch.float32
+    h = x.to(wide) if residual is None else x.to(wide) + residual.to(wide)
+    y = h * torch.rsqrt(h.square().mean(1, keepdim=True) + eps)
+    if weight is not None:
+        y = y * weight.to(wide).reshape(1, -1, *([1] * (x.ndim - 2)))
+    return y.to(x.dtype) if residual is None else (y.to(x.dtype), h.to(x.dtype))
+
+
+# ------------------------------------------------------------------------------------------------------------------
 # layers
 # ------------------------------------------------------------------------------------------------------------------
 def binomial_kernel(taps: Sequence[float] = (1.0, 3.0, 3.0, 1.0)) -> torch.Tensor:
@@ -252,13 +371,17 @@ class ToTexture(nn.Module):
 
 class StyleUNetLite(nn.Module):
     """Encoder: conv -> (Down)* to 8x8.  Decoder: (StyledConv up, StyledConv) per level with the encoder feature of the same
-    resolution merged in by a 3x3 conv, texture accumulated in the Haar domain, synthesised once at the end."""
+    resolution merged in by a 3x3 conv, texture accumulated in the Haar domain, synthesised once at the end.
+    norm="rms": the decoder's second convolution of a level becomes a residual branch, rms_norm(conv(x), gain, residual=x), and
+    the style vector is normalised by rms_norm (None: neither, no gains among the parameters)."""
 
     def __init__(self, size: int = 512, in_ch: int = 4, out_ch: int = 51, style_dim: int = 512, middle: int = 8,
-                 impl: str = "hip", channels=None):
+                 impl: str = "hip", channels=None, norm=None):
         super().__init__()
+        if norm not in (None, "rms"):
+            raise ValueError(f"StyleUNetLite: norm must be None or 'rms', got {norm!r}")
         ch = dict(CHANNELS if channels is None else channels)
-        self.size, self.style_dim, self.impl = size, style_dim, impl
+        self.size, self.style_dim, self.impl, self.norm = size, style_dim, impl, norm
         half = size // 2
         self.mapping = nn.Sequential(nn.Linear(style_dim, style_dim), nn.LeakyReLU(0.2), nn.Linear(style_dim, style_dim))
         self.stem = EqualConv(in_ch, ch[half], 3, impl=impl)
@@ -272,16 +395,23 @@ class StyleUNetLite(nn.Module):
             cin = ch[res]
             self.enc_res.append(res)
         self.ups, self.convs, self.heads = nn.ModuleList(), nn.ModuleList(), nn.ModuleList()
+        if norm:
+            self.gains = nn.ParameterList()
         while res < half:
             res *= 2
             self.ups.append(StyledConv(cin, ch[res], style_dim, up=True, impl=impl))
             self.merges.append(EqualConv(2 * ch[res], ch[res], 3, impl=impl))
             self.convs.append(StyledConv(ch[res], ch[res], style_dim, impl=impl))
             self.heads.append(ToTexture(ch[res], out_ch, impl=impl))
+            if norm:
+                self.gains.append(nn.Parameter(torch.ones(ch[res])))
             cin = ch[res]
 
     def forward(self, cond, style):
-        w = self.mapping(F.normalize(style, dim=1) * math.sqrt(style.shape[1]))
+        if self.norm:
+            w = self.mapping(rms_norm(style, impl=self.impl))
+        else:
+            w = self.mapping(F.normalize(style, dim=1) * math.sqrt(style.shape[1]))
         x = self.stem_down(self.stem(cond))
         skips = [x]
         for d in self.downs:
@@ -291,7 +421,7 @@ class StyleUNetLite(nn.Module):
         for i, (up, merge, conv, head) in enumerate(zip(self.ups, self.merges, self.convs, self.heads)):
             x = up(x, w)
             x = merge(torch.cat([x, skips[-2 - i]], 1))
-            x = conv(x, w)
+            x = rms_norm(conv(x, w), self.gains[i], residual=x, impl=self.impl)[0] if self.norm else conv(x, w)
             tex = head(x, tex)
         return self.heads[-1].haar_up(tex)                 # [B, out_ch, size, size]
 

@@ -287,6 +287,7 @@ int ggs_dist2_3nn_grid(int P, const float* points, float* out, void* scratch, vo
 #define GGS_DTYPE_F32 0
 #define GGS_DTYPE_F16 1
 #define GGS_DTYPE_F64 2
+#define GGS_DTYPE_BF16 3   /* ggs_rms_norm_* and ggs_grad_* only */
 int ggs_fused_bias_act_t(int dtype, size_t n, const void* x, const void* bias, const void* ref, int step_b, int size_b,
                          int act, int grad, float alpha, float scale, void* y, void* stream);
 int ggs_upfirdn2d_t(int dtype, int major, int in_h, int in_w, int minor, const void* input, const void* kernel, int kh,
@@ -299,6 +300,26 @@ int ggs_upfirdn2d_out_size(int in_h, int in_w, int kh, int kw, int up_x, int up_
 int ggs_upfirdn2d(int major, int in_h, int in_w, int minor, const float* input, const float* kernel, int kh, int kw,
                   int up_x, int up_y, int down_x, int down_y, int pad_x0, int pad_x1, int pad_y0, int pad_y1,
                   float* out, void* stream);
+
+/*
+ * Root-mean-square norm over the channels of a feature map, with the residual's addition: the pixel norm of StyleGAN-type
+ * networks (ggsplat.stylenet; no reference counterpart).  Layout [outer][channels][inner], element (o, c, i) at
+ * (o channels + c) inner + i: inner = H W for channels-first maps, 1 for rows of `channels` contiguous values.
+ *   forward:  h = x + residual (residual NULL: h = x);  q = 1 / sqrt(mean over c of h^2 + eps), eps > 0;  y = weight[c] q h.
+ *             `h` (NULL: not stored) and `q` [outer][inner] (NULL: not stored; float, double for GGS_DTYPE_F64) are what the
+ *             backward pass needs.  The norm is that of the sum before `h` is rounded to the element type.
+ *   backward: dx = dL/dx = dL/dresidual from gy = dL/dy and gh = dL/dh (NULL: none); dw [channels] = dL/dweight (NULL: not
+ *             computed).  x, residual: as in the forward call, or x = h and residual = NULL (exact in float and double).
+ * dtype GGS_DTYPE_*: the type of x, residual, y, h, gy, gh, dx.  weight (NULL: 1) and dw have that type too, or float where
+ * weight_f32 != 0.  Sums in float (double for GGS_DTYPE_F64), in an order that does not depend on scheduling.
+ * Tensors need no alignment beyond their element's.  workspace (needed with dw): ggs_rms_norm_workspace_bytes(...), any content.
+ */
+int ggs_rms_norm_forward(int dtype, size_t outer, int channels, size_t inner, const void* x, const void* residual,
+                         const void* weight, int weight_f32, double eps, void* y, void* h, void* q, void* stream);
+size_t ggs_rms_norm_workspace_bytes(int dtype, size_t outer, int channels, size_t inner);
+int ggs_rms_norm_backward(int dtype, size_t outer, int channels, size_t inner, const void* x, const void* residual,
+                          const void* weight, int weight_f32, const void* q, const void* gy, const void* gh, void* dx,
+                          void* dw, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Optimiser update of the inner loops as graph-capturable kernels -- what the reference does with
@@ -331,6 +352,29 @@ int ggs_adam_tick_step_multi(int n_tensors, const size_t* numel, float* const* p
                              float* const* exp_avgs, float* const* exp_avg_sqs, const float* const* lrs,
                              void* const* states, double beta1, double beta2, double eps, const void* guard,
                              void* stream);
+
+/*
+ * Global gradient norm N = sqrt(sum over all tensors and elements of g^2) and clipping by it (no reference counterpart; the
+ * semantics of torch.nn.utils.clip_grad_norm_): factor c = min(1, max_norm / (N + 1e-6)), NaN where N is NaN, max_norm >= 0.
+ *   ggs_grad_norm:      *norm = N.
+ *   ggs_grad_clip:      *norm = N, then every gradient *= c in place (c = 1: nothing is written).  No two tensors may overlap.
+ *   ggs_adam_clip_step: *norm = N, then ggs_adam_tick_step_multi (tick != 0) / ggs_adam_step_multi (tick = 0) on the gradients
+ *                       times c; the gradients themselves stay as they are.  Float only, 16-byte aligned, each tensor listed
+ *                       once.  A non-zero *guard voids the step: parameters, moments, states and *norm are left as they were.
+ * Any number of tensors (host arrays of n_tensors sizes / device pointers); empty ones are skipped, none at all gives N = 0.
+ * dtypes [n_tensors]: GGS_DTYPE_F32 / _F16 / _BF16, NULL: all float; tensors need no alignment beyond their element's.
+ * norm: one device float.  Sums in double, in a fixed order.  workspace: ggs_grad_norm_workspace_bytes(n_tensors) bytes, 8-byte
+ * aligned, any content; calls that may run at the same time need one each.
+ */
+size_t ggs_grad_norm_workspace_bytes(int n_tensors);
+int ggs_grad_norm(int n_tensors, const size_t* numel, const void* const* grads, const int* dtypes, float* norm,
+                  void* workspace, size_t workspace_bytes, void* stream);
+int ggs_grad_clip(int n_tensors, const size_t* numel, void* const* grads, const int* dtypes, double max_norm, float* norm,
+                  void* workspace, size_t workspace_bytes, void* stream);
+int ggs_adam_clip_step(int n_tensors, const size_t* numel, float* const* params, const float* const* grads,
+                       float* const* exp_avgs, float* const* exp_avg_sqs, const float* const* lrs, void* const* states,
+                       double beta1, double beta2, double eps, double max_norm, int tick, const void* guard, float* norm,
+                       void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * The rest of one s2 registration iteration in two kernels: hinge regularisers of the first-frame
