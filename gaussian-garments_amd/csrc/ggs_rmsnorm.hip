@@ -25,7 +25,7 @@ template <typename T> struct NormArgs {
     const T *x, *r, *gy, *gh;
     const void* w;
     bool w32;                    // w (and dw) are float whatever T is
-    A eps;
+    A eps, inv_c;                // 1 / C
     T *y, *h, *dx;
     A* q;                        // [outer][inner]
     A* partial;                  // [n_partial][C]
@@ -134,22 +134,381 @@ __global__ __launch_bounds__(256) void k_rms_dw(NormArgs<T> a) {
     }
 }
 
-// dw[c] = sum of the partials, 64 channels a workgroup
+// dw[c] = sum of the partials, 16 channels a workgroup, 64 rows of partials at a time
 template <typename T>
-__global__ __launch_bounds__(256) void k_rms_dw_sum(NormArgs<T> a) {
+__global__ __launch_bounds__(1024) void k_rms_dw_sum(NormArgs<T> a) {
     typedef typename Acc<T>::type A;
-    __shared__ A lds[256];
-    const int c = blockIdx.x * 64 + (threadIdx.x & 63);
+    __shared__ A lds[64][17];
+    const int lc = threadIdx.x & 15, row = threadIdx.x >> 4, c = blockIdx.x * 16 + lc;
     A s = 0;
-    if (c < a.C) for (int k = threadIdx.x >> 6; k < a.n_partial; k += 4) s += a.partial[(size_t)k * a.C + c];
-    s = sum_waves<A>(s, lds);
-    if (c < a.C && threadIdx.x < 64) {
+    if (c < a.C) for (int k = row; k < a.n_partial; k += 64) s += a.partial[(size_t)k * a.C + c];
+    lds[row][lc] = s;
+    __syncthreads();
+    if (row) return;
+    s = 0;
+#pragma unroll
+    for (int k = 0; k < 64; ++k) s += lds[k][lc];
+    if (c < a.C) {
         if (a.w32) static_cast<float*>(a.dw)[c] = (float)s;
         else static_cast<T*>(a.dw)[c] = (T)s;
     }
 }
 
-int partials(size_t pixels) { return (int)(pixels < 64 * 256 ? (pixels + 255) / 256 : 64); }
+// ---- one pass over the data: a pixel's channels stay in registers ----------------------------------------------------------
+// VEC elements at any element address as one access (unaligned accesses are legal on this part).  Addresses are a base that is
+// the same for the whole workgroup plus 32-bit byte offsets a lane, which all tensors of a pixel share.
+template <typename T, int VEC> struct __attribute__((packed, aligned(alignof(T)))) Pack { T v[VEC]; };
+template <typename T, int VEC> __device__ __forceinline__ Pack<T, VEC> fetch(const T* base, unsigned off) {
+    return *reinterpret_cast<const Pack<T, VEC>*>(reinterpret_cast<const char*>(base) + off);
+}
+template <typename T, int VEC> __device__ __forceinline__ void put(T* base, unsigned off, const float (&v)[VEC]) {
+    Pack<T, VEC> o;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) o.v[j] = (T)v[j];
+    *reinterpret_cast<Pack<T, VEC>*>(reinterpret_cast<char*>(base) + off) = o;
+}
+template <typename T, int VEC> __device__ __forceinline__ void fetch_sum(const NormArgs<T>& a, size_t base, unsigned off, float (&h)[VEC]) {
+    const Pack<T, VEC> x = fetch<T, VEC>(a.x + base, off);
+    if (a.r) {
+        const Pack<T, VEC> r = fetch<T, VEC>(a.r + base, off);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) h[j] = (float)x.v[j] + (float)r.v[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) h[j] = (float)x.v[j];
+    }
+}
+
+// Channels-first maps.  A workgroup takes LP VEC neighbouring pixels of one map and all their channels: LP lanes of a wave lie
+// along the pixels, its other 64 / LP lanes and the waves along the channels, K channels a thread.  The last tile of a map is
+// moved back to end with the map: pixels that two tiles hold get the same values from both, and count once in dw.
+template <int VEC, int LP> struct PlaneTile {
+    static constexpr int LC = 64 / LP, TP = LP * VEC;
+    int c0, step;                            // first channel of this thread, channel step
+    size_t base, q_base, stride;             // of the map; elements from one of this thread's channels to the next
+    unsigned i0;                             // first pixel of this lane's vector
+    int fresh;                               // its first pixel that no vector before holds
+    template <typename T> __device__ __forceinline__ PlaneTile(const NormArgs<T>& a, unsigned tile) {
+        const unsigned tiles = ((unsigned)a.inner + TP - 1) / TP, o = tile / tiles;
+        const int lane = threadIdx.x & 63;
+        const unsigned i = (tile - o * tiles) * TP + (lane % LP) * VEC, last = (unsigned)a.inner - VEC;
+        i0 = i < last ? i : last;
+        fresh = (int)(i - i0 < (unsigned)VEC ? i - i0 : VEC);
+        c0 = (threadIdx.x >> 6) * LC + lane / LP;
+        step = (blockDim.x >> 6) * LC;
+        base = (size_t)o * a.C * a.inner;
+        q_base = (size_t)o * a.inner;
+        stride = (size_t)step * a.inner;
+    }
+    template <typename T> __device__ __forceinline__ unsigned off(const NormArgs<T>& a) const {
+        return ((unsigned)c0 * (unsigned)a.inner + i0) * (unsigned)sizeof(T);
+    }
+};
+
+// Sums over the lanes of a wave that hold the same pixels, then over the waves.
+template <int VEC, int LP> __device__ __forceinline__ void sum_channels(float (&s)[VEC], float* lds) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+#pragma unroll
+    for (int d = LP; d < 64; d <<= 1) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) s[j] += __shfl_xor(s[j], d);
+    }
+    if (waves == 1) return;
+    if (lane < LP) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) lds[(wave * LP + lane) * VEC + j] = s[j];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) s[j] = 0.0f;
+#pragma unroll 2
+    for (int k = 0; k < waves; ++k) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) s[j] += lds[(k * LP + lane % LP) * VEC + j];
+    }
+}
+
+template <typename T, int VEC, int LP, int K>
+__global__ __launch_bounds__(1024) void k_planes_forward(NormArgs<T> a) {
+    __shared__ float lds[16 * LP * VEC];
+    const PlaneTile<VEC, LP> t(a, blockIdx.x);
+    const unsigned off = t.off(a);
+    float h[K][VEC], s[VEC] = {};
+#pragma unroll
+    for (int k = 0; k < K; ++k) if (t.c0 + k * t.step < a.C) fetch_sum<T, VEC>(a, t.base + k * t.stride, off, h[k]);
+#pragma unroll
+    for (int k = 0; k < K; ++k) if (t.c0 + k * t.step < a.C) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) s[j] = fmaf(h[k][j], h[k][j], s[j]);
+    }
+    sum_channels<VEC, LP>(s, lds);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) s[j] = rsqrtf(s[j] * a.inv_c + a.eps);
+    if (t.c0 == 0 && a.q) put<float, VEC>(a.q + t.q_base, t.i0 * 4u, s);
+#pragma unroll
+    for (int k = 0; k < K; ++k) if (t.c0 + k * t.step < a.C) {
+        const float w = weight(a, t.c0 + k * t.step);
+        float y[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) y[j] = w * (h[k][j] * s[j]);
+        if (a.h) put<T, VEC>(a.h + t.base + k * t.stride, off, h[k]);
+        put<T, VEC>(a.y + t.base + k * t.stride, off, y);
+    }
+}
+
+// A workgroup walks tiles with a fixed stride and keeps its share of dw in registers meanwhile: one row of partials each.
+template <typename T, int VEC, int LP, int K>
+__global__ __launch_bounds__(1024) void k_planes_backward(NormArgs<T> a, unsigned tiles) {
+    __shared__ float lds[2][16 * LP * VEC];
+    constexpr bool EARLY = K * VEC <= 16;    // gh on its way with the rest, where the registers allow it
+    float dw[K] = {};
+    int turn = 0;
+    for (unsigned tile = blockIdx.x; tile < tiles; tile += gridDim.x, turn ^= 1) {
+        const PlaneTile<VEC, LP> t(a, tile);
+        const unsigned off = t.off(a);
+        float h[K][VEC], g[K][VEC], s[VEC] = {};
+        Pack<T, VEC> gh[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) if (t.c0 + k * t.step < a.C) {
+            const size_t base = t.base + k * t.stride;
+            fetch_sum<T, VEC>(a, base, off, h[k]);
+            const Pack<T, VEC> p = fetch<T, VEC>(a.gy + base, off);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) g[k][j] = (float)p.v[j];
+            if (EARLY && a.gh) gh[k] = fetch<T, VEC>(a.gh + base, off);
+        }
+        const Pack<float, VEC> q = fetch<float, VEC>(a.q + t.q_base, t.i0 * 4u);
+#pragma unroll
+        for (int k = 0; k < K; ++k) if (t.c0 + k * t.step < a.C) {
+            const float w = weight(a, t.c0 + k * t.step);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                h[k][j] *= q.v[j];
+                const float gn = g[k][j] * h[k][j];
+                dw[k] += j >= t.fresh ? gn : 0.0f;
+                s[j] = fmaf(w, gn, s[j]);
+                g[k][j] *= w;
+            }
+        }
+        sum_channels<VEC, LP>(s, lds[turn]);
+#pragma unroll
+        for (int k = 0; k < K; ++k) if (t.c0 + k * t.step < a.C) {
+            float d[VEC];
+            if (!EARLY && a.gh) gh[k] = fetch<T, VEC>(a.gh + t.base + k * t.stride, off);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                d[j] = q.v[j] * (g[k][j] - h[k][j] * (s[j] * a.inv_c));
+                if (a.gh) d[j] += (float)gh[k].v[j];
+            }
+            put<T, VEC>(a.dx + t.base + k * t.stride, off, d);
+        }
+    }
+    if (!a.dw) return;
+    constexpr int LC = 64 / LP;
+    const int lane = threadIdx.x & 63, c0 = (threadIdx.x >> 6) * LC + lane / LP, step = (blockDim.x >> 6) * LC;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+#pragma unroll
+        for (int d = 1; d < LP; d <<= 1) dw[k] += __shfl_xor(dw[k], d);
+        if (lane % LP == 0 && c0 + k * step < a.C) a.partial[(size_t)blockIdx.x * a.C + c0 + k * step] = dw[k];
+    }
+}
+
+// Rows of contiguous channels: G lanes a row, K vectors of VEC channels a lane.  The last vector of a row is moved back to end
+// with the row: channels that two vectors hold count once in the sums.
+template <int VEC, int G> struct RowSlot {
+    int lane;                                // within the row's lanes
+    __device__ __forceinline__ RowSlot() : lane(threadIdx.x % G) {}
+    __device__ __forceinline__ bool on(int k, int C) const { return (lane + k * G) * VEC < C; }
+    __device__ __forceinline__ int at(int k, int C) const { const int c = (lane + k * G) * VEC; return c < C - VEC ? c : C - VEC; }
+    __device__ __forceinline__ int fresh(int k, int C) const { return (lane + k * G) * VEC - at(k, C); }
+};
+
+// Sum over the G lanes of a row (rows of more than a wave: G / 64 waves, `lds` one float a wave of the workgroup).
+template <int G> __device__ __forceinline__ float sum_row(float s, float* lds) {
+#pragma unroll
+    for (int d = 1; d < (G < 64 ? G : 64); d <<= 1) s += __shfl_xor(s, d);
+    if (G > 64) {
+        const int wave = threadIdx.x >> 6, first = wave / (G / 64) * (G / 64);
+        if ((threadIdx.x & 63) == 0) lds[wave] = s;
+        __syncthreads();
+        s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < G / 64; ++k) s += lds[first + k];
+    }
+    return s;
+}
+
+template <typename T, int VEC> __device__ __forceinline__ void weights(const NormArgs<T>& a, int c, float (&w)[VEC]) {
+    if (!a.w) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) w[j] = 1.0f;
+    } else if (a.w32) {
+        const Pack<float, VEC> p = fetch<float, VEC>(static_cast<const float*>(a.w), c * 4u);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) w[j] = p.v[j];
+    } else {
+        const Pack<T, VEC> p = fetch<T, VEC>(static_cast<const T*>(a.w), c * (unsigned)sizeof(T));
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) w[j] = (float)p.v[j];
+    }
+}
+
+template <typename T, int VEC, int G, int K>
+__global__ __launch_bounds__(G > 256 ? G : 256) void k_rows_forward(NormArgs<T> a) {
+    constexpr int THREADS = G > 256 ? G : 256, ROWS = THREADS / G;
+    __shared__ float lds[16];
+    const RowSlot<VEC, G> t;
+    const size_t row0 = (size_t)blockIdx.x * ROWS, base = row0 * a.C;
+    const unsigned row = threadIdx.x / G;
+    const bool in = row0 + row < a.outer;
+    float h[K][VEC], s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) if (in && t.on(k, a.C)) fetch_sum<T, VEC>(a, base, (row * a.C + t.at(k, a.C)) * (unsigned)sizeof(T), h[k]);
+#pragma unroll
+    for (int k = 0; k < K; ++k) if (in && t.on(k, a.C)) {
+        const int fresh = t.fresh(k, a.C);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) s = j >= fresh ? fmaf(h[k][j], h[k][j], s) : s;
+    }
+    s = sum_row<G>(s, lds);
+    const float q = rsqrtf(s * a.inv_c + a.eps);
+    if (in && t.lane == 0 && a.q) a.q[row0 + row] = q;
+#pragma unroll
+    for (int k = 0; k < K; ++k) if (in && t.on(k, a.C)) {
+        const int c = t.at(k, a.C);
+        float w[VEC], y[VEC];
+        weights<T, VEC>(a, c, w);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) y[j] = w[j] * (h[k][j] * q);
+        if (a.h) put<T, VEC>(a.h + base, (row * a.C + c) * (unsigned)sizeof(T), h[k]);
+        put<T, VEC>(a.y + base, (row * a.C + c) * (unsigned)sizeof(T), y);
+    }
+}
+
+// A workgroup of 1024 threads walks sets of 1024 / G rows and keeps its share of dw in registers meanwhile.
+template <typename T, int VEC, int G, int K>
+__global__ __launch_bounds__(1024) void k_rows_backward(NormArgs<T> a, unsigned sets) {
+    constexpr int ROWS = 1024 / G;
+    __shared__ float lds[2][16], sum[G * K * VEC];
+    const RowSlot<VEC, G> t;
+    const unsigned row = threadIdx.x / G;
+    float dw[K][VEC] = {};
+    int turn = 0;
+    for (unsigned set = blockIdx.x; set < sets; set += gridDim.x, turn ^= 1) {
+        const size_t row0 = (size_t)set * ROWS, base = row0 * a.C;
+        const bool in = row0 + row < a.outer;
+        float h[K][VEC], g[K][VEC], s = 0.0f;
+        Pack<T, VEC> gh[K];
+        const float q = in ? a.q[row0 + row] : 0.0f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) if (in && t.on(k, a.C)) {
+            const unsigned off = (row * a.C + t.at(k, a.C)) * (unsigned)sizeof(T);
+            fetch_sum<T, VEC>(a, base, off, h[k]);
+            const Pack<T, VEC> p = fetch<T, VEC>(a.gy + base, off);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) g[k][j] = (float)p.v[j];
+            if (a.gh) gh[k] = fetch<T, VEC>(a.gh + base, off);
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k) if (in && t.on(k, a.C)) {
+            const int fresh = t.fresh(k, a.C);
+            float w[VEC];
+            weights<T, VEC>(a, t.at(k, a.C), w);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                h[k][j] *= q;
+                const float gn = g[k][j] * h[k][j];
+                dw[k][j] += gn;
+                g[k][j] *= w[j];
+                s = j >= fresh ? fmaf(w[j], gn, s) : s;
+            }
+        }
+        s = sum_row<G>(s, lds[turn]) * a.inv_c;
+#pragma unroll
+        for (int k = 0; k < K; ++k) if (in && t.on(k, a.C)) {
+            float d[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                d[j] = q * (g[k][j] - h[k][j] * s);
+                if (a.gh) d[j] += (float)gh[k].v[j];
+            }
+            put<T, VEC>(a.dx + base, (row * a.C + t.at(k, a.C)) * (unsigned)sizeof(T), d);
+        }
+    }
+    if (!a.dw) return;
+    // the rows of one wave by shuffles, then the waves one after the other in LDS (a fixed order)
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+#pragma unroll
+            for (int d = G; d < 64; d <<= 1) dw[k][j] += __shfl_xor(dw[k][j], d);
+        }
+    }
+    constexpr int TURNS = G < 64 ? 16 : ROWS;
+    const int mine = G < 64 ? threadIdx.x >> 6 : threadIdx.x / G;
+    const bool first = G >= 64 || (threadIdx.x & 63) < G;
+    for (int r = 0; r < TURNS; ++r) {
+        if (r == mine && first) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    float* at = sum + (k * G + t.lane) * VEC + j;
+                    *at = r ? *at + dw[k][j] : dw[k][j];
+                }
+            }
+        }
+        __syncthreads();
+    }
+    // vector v holds channels v VEC ... but the last one, which ends with the row
+    const int vecs = (a.C + VEC - 1) / VEC;
+    for (int c = threadIdx.x; c < a.C; c += 1024) {
+        const int v = c / VEC, j = v == vecs - 1 ? c - (a.C - VEC) : c % VEC;
+        a.partial[(size_t)blockIdx.x * a.C + c] = sum[v * VEC + j];
+    }
+}
+
+// ---- which kernel ----------------------------------------------------------------------------------------------------------
+// One-pass kernels: float and 16-bit types, a pixel's channels within the registers of one workgroup (1024 channels of a map,
+// 2048 vectors of a row), a map within 32-bit offsets; the two-pass kernels serve double and what is left.
+struct Plan {
+    int kind;                    // 0 two passes, 1 planes, 2 rows
+    int vec, lanes, k, waves;    // planes: LP and waves of a workgroup; rows: G
+    size_t tiles;                // planes: tiles of all maps; rows: sets of 1024 / G rows
+    int partials;
+};
+
+template <typename T> Plan plan(size_t outer, int C, size_t inner) {
+    Plan p = {};
+    constexpr int FULL = 16 / sizeof(T);
+    const size_t pixels = outer * inner;
+    p.partials = (int)(pixels < 64 * 256 ? (pixels + 255) / 256 : 64);
+    if (sizeof(T) == 8) return p;
+    if (inner == 1) {
+        const int vec = C >= FULL ? FULL : 1, vecs = (C + vec - 1) / vec;
+        const int lanes = vecs <= 8 ? 4 : vecs <= 32 ? 16 : vecs <= 128 ? 64 : vecs <= 512 ? 256 : 1024;
+        const size_t sets = (outer + 1024 / lanes - 1) / (1024 / lanes);
+        if (vecs > 2048 || sets > 0x7fffffffu / 4) return p;          // (the forward kernel's workgroups take a quarter of a set)
+        p.kind = 2; p.vec = vec; p.lanes = lanes; p.k = vecs <= lanes ? 1 : 2; p.tiles = sets;
+        p.partials = (int)(sets < 512 ? sets : 512);
+        return p;
+    }
+    if (C > 1024 || (size_t)C * inner > 0xffffffffu / sizeof(T)) return p;
+    p.vec = inner >= (size_t)FULL ? FULL : 1;
+    p.lanes = 64 / FULL;                                       // 64 pixels a tile
+    while (p.lanes > 4 && (p.vec == 1 || C > 64 * 64 / p.lanes || outer * ((inner + p.lanes * FULL - 1) / (p.lanes * FULL)) < 512)) p.lanes /= 2;
+    const int units = (C + 64 / p.lanes - 1) / (64 / p.lanes);
+    p.k = units <= 4 ? 1 : units <= 16 ? 2 : 4;
+    p.waves = (units + p.k - 1) / p.k;
+    p.tiles = outer * ((inner + p.lanes * p.vec - 1) / (p.lanes * p.vec));
+    if (p.tiles > 0x7fffffffu) return p;
+    p.kind = 1;
+    const size_t fill = 8192 / p.waves;
+    p.partials = (int)(p.tiles < fill ? p.tiles : fill);
+    return p;
+}
 
 int launched(const char* who) {
     hipError_t e = hipGetLastError();
@@ -157,28 +516,76 @@ int launched(const char* who) {
     return GGS_OK;
 }
 
+template <typename T, int VEC, int LP, int K> void planes(bool back, const NormArgs<T>& a, const Plan& p, hipStream_t s) {
+    if (back) hipLaunchKernelGGL((k_planes_backward<T, VEC, LP, K>), dim3((unsigned)p.partials), dim3(p.waves * 64), 0, s, a, (unsigned)p.tiles);
+    else hipLaunchKernelGGL((k_planes_forward<T, VEC, LP, K>), dim3((unsigned)p.tiles), dim3(p.waves * 64), 0, s, a);
+}
+template <typename T, int VEC, int LP> void planes(bool back, const NormArgs<T>& a, const Plan& p, hipStream_t s) {
+    if (p.k == 1) planes<T, VEC, LP, 1>(back, a, p, s);
+    else if (p.k == 2) planes<T, VEC, LP, 2>(back, a, p, s);
+    else planes<T, VEC, LP, 4>(back, a, p, s);
+}
+template <typename T, int VEC, int G, int K> void rows(bool back, const NormArgs<T>& a, const Plan& p, hipStream_t s) {
+    constexpr int THREADS = G > 256 ? G : 256, ROWS = THREADS / G;
+    if (back) hipLaunchKernelGGL((k_rows_backward<T, VEC, G, K>), dim3((unsigned)p.partials), dim3(1024), 0, s, a, (unsigned)p.tiles);
+    else hipLaunchKernelGGL((k_rows_forward<T, VEC, G, K>), dim3((unsigned)((a.outer + ROWS - 1) / ROWS)), dim3(THREADS), 0, s, a);
+}
+template <typename T, int VEC, int G> void rows(bool back, const NormArgs<T>& a, const Plan& p, hipStream_t s) {
+    if (p.k == 1) rows<T, VEC, G, 1>(back, a, p, s);
+    else rows<T, VEC, G, 2>(back, a, p, s);
+}
+
+template <typename T> void one_pass(bool back, const NormArgs<T>& a, const Plan& p, hipStream_t s) {
+    constexpr int FULL = 16 / sizeof(T);
+    if (p.kind == 2) {
+        if (p.vec == 1) rows<T, 1, 4>(back, a, p, s);
+        else if (p.lanes == 4) rows<T, FULL, 4>(back, a, p, s);
+        else if (p.lanes == 16) rows<T, FULL, 16>(back, a, p, s);
+        else if (p.lanes == 64) rows<T, FULL, 64>(back, a, p, s);
+        else if (p.lanes == 256) rows<T, FULL, 256>(back, a, p, s);
+        else rows<T, FULL, 1024>(back, a, p, s);
+        return;
+    }
+    if (p.vec == 1) planes<T, 1, 4>(back, a, p, s);
+    else if (p.lanes == 4) planes<T, FULL, 4>(back, a, p, s);
+    else if (p.lanes == 8) planes<T, FULL, 8>(back, a, p, s);
+    else planes<T, FULL, 64 / FULL>(back, a, p, s);
+}
+template <> void one_pass<double>(bool, const NormArgs<double>&, const Plan&, hipStream_t) {}
+
 template <typename T> int run_forward(NormArgs<T> a, hipStream_t s) {
-    const size_t tiles = a.inner == 1 ? 1 : (a.inner + 63) / 64, blocks = a.outer * tiles;
-    if (blocks > 0x7fffffffu) return ggs_fail_(GGS_ERR_SIZE, "ggs_rms_norm_forward: more than 2^31 workgroups");
-    if (a.inner == 1) hipLaunchKernelGGL((k_rms_forward<T, false>), dim3((unsigned)blocks), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((k_rms_forward<T, true>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+    const Plan p = plan<T>(a.outer, a.C, a.inner);
+    const size_t tiles = a.inner == 1 ? 1 : (a.inner + 63) / 64;
+    if (!p.kind && a.outer * tiles > 0x7fffffffu) return ggs_fail_(GGS_ERR_SIZE, "ggs_rms_norm_forward: more than 2^31 workgroups");
+    if (p.kind) one_pass(false, a, p, s);
+    else if (a.inner == 1) hipLaunchKernelGGL((k_rms_forward<T, false>), dim3((unsigned)a.outer), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_rms_forward<T, true>), dim3((unsigned)(a.outer * tiles)), dim3(256), 0, s, a);
     return launched("ggs_rms_norm_forward");
 }
 
 template <typename T> int run_backward(NormArgs<T> a, hipStream_t s) {
-    const size_t tiles = a.inner == 1 ? 1 : (a.inner + 63) / 64, blocks = a.outer * tiles;
-    if (blocks > 0x7fffffffu) return ggs_fail_(GGS_ERR_SIZE, "ggs_rms_norm_backward: more than 2^31 workgroups");
-    if (a.inner == 1) hipLaunchKernelGGL((k_rms_backward<T, false>), dim3((unsigned)blocks), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((k_rms_backward<T, true>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+    const Plan p = plan<T>(a.outer, a.C, a.inner);
+    const size_t tiles = a.inner == 1 ? 1 : (a.inner + 63) / 64;
+    if (!p.kind && a.outer * tiles > 0x7fffffffu) return ggs_fail_(GGS_ERR_SIZE, "ggs_rms_norm_backward: more than 2^31 workgroups");
+    if (p.kind) one_pass(true, a, p, s);
+    else if (a.inner == 1) hipLaunchKernelGGL((k_rms_backward<T, false>), dim3((unsigned)a.outer), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_rms_backward<T, true>), dim3((unsigned)(a.outer * tiles)), dim3(256), 0, s, a);
     int rc = launched("ggs_rms_norm_backward");
     if (rc != GGS_OK || !a.dw) return rc;
-    a.n_partial = partials(a.outer * a.inner);
-    if (a.inner == 1) hipLaunchKernelGGL((k_rms_dw<T, false>), dim3((a.C + 255) / 256, a.n_partial), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((k_rms_dw<T, true>), dim3(a.C, a.n_partial), dim3(256), 0, s, a);
-    rc = launched("ggs_rms_norm_backward");
-    if (rc != GGS_OK) return rc;
-    hipLaunchKernelGGL((k_rms_dw_sum<T>), dim3((a.C + 63) / 64), dim3(256), 0, s, a);
+    a.n_partial = p.partials;
+    if (!p.kind) {
+        if (a.inner == 1) hipLaunchKernelGGL((k_rms_dw<T, false>), dim3((a.C + 255) / 256, a.n_partial), dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((k_rms_dw<T, true>), dim3(a.C, a.n_partial), dim3(256), 0, s, a);
+        rc = launched("ggs_rms_norm_backward");
+        if (rc != GGS_OK) return rc;
+    }
+    hipLaunchKernelGGL((k_rms_dw_sum<T>), dim3((a.C + 15) / 16), dim3(1024), 0, s, a);
     return launched("ggs_rms_norm_backward");
+}
+
+size_t partials(int dtype, size_t outer, int C, size_t inner) {
+    return dtype == GGS_DTYPE_F64 ? plan<double>(outer, C, inner).partials :
+           dtype == GGS_DTYPE_F32 ? plan<float>(outer, C, inner).partials : plan<_Float16>(outer, C, inner).partials;
 }
 
 int check_sizes(const char* who, int dtype, size_t outer, int channels, size_t inner, double eps) {
@@ -195,6 +602,7 @@ NormArgs<T> norm_args(size_t outer, int channels, size_t inner, const void* x, c
     a.outer = outer; a.inner = inner; a.C = channels;
     a.x = static_cast<const T*>(x); a.r = static_cast<const T*>(residual);
     a.w = weight; a.w32 = weight_f32 != 0; a.eps = (typename Acc<T>::type)eps;
+    a.inv_c = (typename Acc<T>::type)1 / channels;
     return a;
 }
 
@@ -238,7 +646,7 @@ int ggs_rms_norm_forward(int dtype, size_t outer, int channels, size_t inner, co
 
 size_t ggs_rms_norm_workspace_bytes(int dtype, size_t outer, int channels, size_t inner) {
     if (channels <= 0 || outer == 0 || inner == 0) return 0;
-    return (size_t)partials(outer * inner) * (size_t)channels * (dtype == GGS_DTYPE_F64 ? 8 : 4);
+    return partials(dtype, outer, channels, inner) * (size_t)channels * (dtype == GGS_DTYPE_F64 ? 8 : 4);
 }
 
 int ggs_rms_norm_backward(int dtype, size_t outer, int channels, size_t inner, const void* x, const void* residual,
