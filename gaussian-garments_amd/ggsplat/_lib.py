@@ -155,21 +155,20 @@ def stream_ptr(dev) -> int:
     return torch.cuda.current_stream(dev).cuda_stream
 
 
-class on_device:
-    """Makes a tensor's device the current one for the launches inside (a launch onto another device's stream is an error)."""
-
-    def __init__(self, dev):
-        self.dev = dev
-
+class _SameDevice:
     def __enter__(self):
-        now = torch.cuda.current_device()
-        self.back = None if self.dev.index in (None, now) else now
-        if self.back is not None:
-            torch.cuda.set_device(self.dev)
+        pass
 
     def __exit__(self, *_):
-        if self.back is not None:
-            torch.cuda.set_device(self.back)
+        pass
+
+
+_same_device = _SameDevice()
+
+
+def on_device(dev):
+    """Context in which `dev` is the current device for the launches inside (a launch onto another device's stream is an error)."""
+    return _same_device if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 def host_mapped_pointer(t) -> int:

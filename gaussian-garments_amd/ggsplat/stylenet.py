@@ -35,7 +35,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from ._lib import check, lib, norm_dtype_code, on_device, ptr, stream_ptr
+from ._lib import check, lib, on_device, ptr, stream_ptr
 
 CHANNELS = {4: 512, 8: 512, 16: 512, 32: 512, 64: 512, 128: 256, 256: 128, 512: 64, 1024: 32, 2048: 16}
 
@@ -155,78 +155,101 @@ def resample2d(x, k, up: int = 1, down: int = 1, pad: Tuple[int, int] = (0, 0), 
 #   h = x + residual,  q = (mean_c h^2 + eps)^-1/2,  y = weight q h;   with n = q h:
 #   dL/dh = q (weight gy - n mean_c(weight gy n)) + gh = dL/dx = dL/dresidual,   dL/dweight = sum over pixels of gy n
 # ------------------------------------------------------------------------------------------------------------------
-_RMS_TYPES = (torch.float32, torch.float16, torch.bfloat16, torch.float64)
+_RMS_TYPES = {torch.float32: 0, torch.float16: 1, torch.float64: 2, torch.bfloat16: 3}      # GGS_DTYPE_*
 
 
 def _rms_layout(x):
-    """(x as the kernels read it, outer, inner, how to bring another tensor of its shape to the same order): channels-last
-    maps and anything else whose channels are innermost are rows, the rest is [B][C][pixels]."""
-    b, c = x.shape[0], x.shape[1]
-    pixels = 1
-    for s in x.shape[2:]:
-        pixels *= s
+    """(x as the kernels read it, outer, inner, whether channels are innermost): channels-last maps and whatever else keeps the
+    channels of a pixel together are rows, the rest is [B][C][pixels]."""
     if x.is_contiguous():
-        return x, (b, pixels), lambda t: t.contiguous()
-    if x.movedim(1, -1).is_contiguous():
-        return x, (b * pixels, 1), lambda t: t if t.movedim(1, -1).is_contiguous() else t.movedim(1, -1).contiguous().movedim(-1, 1)
-    return x.contiguous(), (b, pixels), lambda t: t.contiguous()
+        rows = False
+    else:
+        rows = x.movedim(1, -1).is_contiguous()
+        if not rows:
+            x = x.contiguous()
+    shape = x.shape
+    inner = 1
+    for s in shape[2:]:
+        inner *= s
+    return (x, shape[0] * inner, 1, True) if rows else (x, shape[0], inner, False)
+
+
+def _rms_order(t, rows):
+    """Another tensor of x's shape in the order the kernels read x in."""
+    if not rows:
+        return t.contiguous()
+    return t if t.movedim(1, -1).is_contiguous() else t.movedim(1, -1).contiguous().movedim(-1, 1)
 
 
 def _rms_forward(x, weight, residual, eps, store):
-    """(y, h or None, q or None, x and residual in the kernels' order, layout)."""
-    x, (outer, inner), order = _rms_layout(x)
+    """(y, h or None, x, residual and weight in the kernels' order, q or None, (type, outer, channels, inner, 32-bit weight, rows))"""
+    x, outer, inner, rows = _rms_layout(x)
     y = torch.empty_like(x)
-    h = q = None
+    h = q = hp = rp = qp = None
     if residual is not None:
-        residual = order(residual)
+        residual = _rms_order(residual, rows)
         h = torch.empty_like(x)
+        hp, rp = h.data_ptr(), residual.data_ptr()
+    dev, dtype, c = x.device, x.dtype, x.shape[1]
     if store:
-        q = torch.empty(outer * inner, device=x.device, dtype=torch.float64 if x.dtype is torch.float64 else torch.float32)
-    w = None if weight is None else weight.contiguous()
-    with on_device(x.device):
-        check(lib().ggs_rms_norm_forward(norm_dtype_code(x.dtype), outer, x.shape[1], inner, x.data_ptr(),
-                                         None if residual is None else residual.data_ptr(), ptr(w),
-                                         int(w is not None and w.dtype is torch.float32), eps, y.data_ptr(),
-                                         None if h is None else h.data_ptr(), ptr(q), stream_ptr(x.device)), "ggs_rms_norm_forward")
-    return y, h, q, x, residual, w
+        q = torch.empty(outer * inner, device=dev, dtype=torch.float64 if dtype is torch.float64 else torch.float32)
+        qp = q.data_ptr()
+    w32 = False
+    if weight is not None:
+        weight = weight.contiguous()
+        w32 = weight.dtype is torch.float32
+    plan = (_RMS_TYPES[dtype], outer, c, inner, w32, rows)
+    with on_device(dev):
+        check(lib().ggs_rms_norm_forward(plan[0], outer, c, inner, x.data_ptr(), rp, ptr(weight), w32, eps, y.data_ptr(), hp, qp,
+                                         stream_ptr(dev)), "ggs_rms_norm_forward")
+    return y, h, x, residual, weight, q, plan
 
 
 class _RmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
-        y, h, q, x, residual, w = _rms_forward(x, weight, residual, eps, True)
+        y, h, x, residual, weight, q, ctx.plan = _rms_forward(x, weight, residual, eps, True)
         ctx.set_materialize_grads(False)
+        if h is None:
+            ctx.save_for_backward(x, None, weight, q)
+            return y
         # float and double keep the sum; 16 bits keep both summands, because h is stored rounded (csrc/ggs_rmsnorm.hip)
-        if residual is not None and x.dtype in (torch.float32, torch.float64):
-            ctx.save_for_backward(h, None, w, q)
+        if ctx.plan[0] in (0, 2):
+            ctx.save_for_backward(h, None, weight, q)
         else:
-            ctx.save_for_backward(x, residual, w, q)
-        return y if residual is None else (y, h)
+            ctx.save_for_backward(x, residual, weight, q)
+        return y, h
 
     @staticmethod
     def backward(ctx, gy, gh=None):
         if torch.is_grad_enabled():                                   # create_graph=True
             raise RuntimeError("rms_norm: its gradients are not differentiable again (create_graph=True)")
-        x, residual, w, q = ctx.saved_tensors
+        need = ctx.needs_input_grad
         if gy is None:                                                # only h was used further on
-            return gh, None, gh if ctx.needs_input_grad[2] else None, None
-        x, (outer, inner), order = _rms_layout(x)
-        gy, gh = order(gy), None if gh is None else order(gh)
+            return gh, None, gh if need[2] else None, None
+        x, residual, w, q = ctx.saved_tensors
+        code, outer, c, inner, w32, rows = ctx.plan
+        gy = _rms_order(gy, rows)
+        gp = rp = dw = dwp = wp = None
+        if gh is not None:
+            gh = _rms_order(gh, rows)
+            gp = gh.data_ptr()
+        if residual is not None:
+            rp = residual.data_ptr()
         dx = torch.empty_like(x)
-        L, code, dw, ws, nb = lib(), norm_dtype_code(x.dtype), None, None, 0
-        with on_device(x.device):
-            if ctx.needs_input_grad[1]:
+        dev, nb, L = x.device, 0, lib()
+        with on_device(dev):
+            if need[1]:
                 dw = torch.empty_like(w)
-                nb = int(L.ggs_rms_norm_workspace_bytes(code, outer, x.shape[1], inner))
-                ws = torch.empty(nb, dtype=torch.uint8, device=x.device)
-                if x.numel() == 0:
-                    dw.zero_()
-            check(L.ggs_rms_norm_backward(code, outer, x.shape[1], inner, x.data_ptr(),
-                                          None if residual is None else residual.data_ptr(), ptr(w),
-                                          int(w is not None and w.dtype is torch.float32), ptr(q), gy.data_ptr(),
-                                          None if gh is None else gh.data_ptr(), dx.data_ptr(), ptr(dw), ptr(ws), nb,
-                                          stream_ptr(x.device)), "ggs_rms_norm_backward")
-        return dx, dw, dx if ctx.needs_input_grad[2] else None, None
+                nb = L.ggs_rms_norm_workspace_bytes(code, outer, c, inner)
+                if nb:
+                    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+                    dwp, wp = dw.data_ptr(), ws.data_ptr()
+                else:
+                    dw.zero_()                                        # no pixels
+            check(L.ggs_rms_norm_backward(code, outer, c, inner, x.data_ptr(), rp, ptr(w), w32, q.data_ptr(), gy.data_ptr(), gp,
+                                          dx.data_ptr(), dwp, wp, nb, stream_ptr(dev)), "ggs_rms_norm_backward")
+        return dx, dw, dx if need[2] else None, None
 
 
 def rms_norm(x, weight=None, residual=None, eps: float = 1e-8, impl: str = "hip"):
@@ -235,13 +258,14 @@ def rms_norm(x, weight=None, residual=None, eps: float = 1e-8, impl: str = "hip"
     x, residual: float32 / float16 / bfloat16 / float64, the same shape; weight [C]: x's type or float32; contiguous and
     channels-last maps are taken as they are.  The norm is that of the unrounded sum; sums are in float (double for float64).
     Differentiable once (its gradients are not differentiable again)."""
-    if x.ndim < 2 or x.shape[1] == 0:
-        raise ValueError(f"rms_norm: x must be [B, C, ...] with C > 0, got {tuple(x.shape)}")
-    if x.dtype not in _RMS_TYPES:
-        raise TypeError(f"rms_norm: {x.dtype} is not float32, float16, bfloat16 or float64")
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
+    shape, dtype = x.shape, x.dtype
+    if len(shape) < 2 or shape[1] == 0:
+        raise ValueError(f"rms_norm: x must be [B, C, ...] with C > 0, got {tuple(shape)}")
+    if dtype not in _RMS_TYPES:
+        raise TypeError(f"rms_norm: {dtype} is not float32, float16, bfloat16 or float64")
+    if residual is not None and (residual.shape != shape or residual.dtype is not dtype or residual.device != x.device):
         raise ValueError("rms_norm: residual must have x's shape, type and device")
-    if weight is not None and (weight.shape != (x.shape[1],) or weight.dtype not in (x.dtype, torch.float32) or weight.device != x.device):
+    if weight is not None and (weight.shape != shape[1:2] or weight.dtype not in (dtype, torch.float32) or weight.device != x.device):
         raise ValueError("rms_norm: weight must be [C], of x's type or float32, on x's device")
     eps = float(eps)
     if not (eps > 0.0 and math.isfinite(eps)):
