@@ -174,6 +174,17 @@ template <typename T, int VEC, bool NT = false> __device__ __forceinline__ Pack<
         return *reinterpret_cast<const Pack<T, VEC>*>(at);
     }
 }
+// A pack that stays in registers between phases: as four words, where the compiler would give every 16-bit element one
+template <typename T, int VEC, bool WIDE = sizeof(T) * VEC == 16> struct Kept {
+    Bits16 b;
+    __device__ __forceinline__ void operator=(const Pack<T, VEC>& p) { __builtin_memcpy(&b, &p, 16); }
+    __device__ __forceinline__ Pack<T, VEC> get() const { Pack<T, VEC> p; __builtin_memcpy(&p, &b, 16); return p; }
+};
+template <typename T, int VEC> struct Kept<T, VEC, false> {
+    Pack<T, VEC> p;
+    __device__ __forceinline__ void operator=(const Pack<T, VEC>& o) { p = o; }
+    __device__ __forceinline__ Pack<T, VEC> get() const { return p; }
+};
 // Whole 16-byte vectors are stored past the caches: what they would push out are the inputs that other workgroups are about to
 // read (4096 x 4096 bf16 forward 29.3 -> 22.0 us, 256 x 128 x 128 float backward 16.8 -> 15.5 us).
 template <typename T, int VEC> __device__ __forceinline__ void put(T* base, unsigned off, const float (&v)[VEC]) {
@@ -189,15 +200,28 @@ template <typename T, int VEC> __device__ __forceinline__ void put(T* base, unsi
         *reinterpret_cast<Pack<T, VEC>*>(at) = o;
     }
 }
-template <typename T, int VEC, bool NT = false> __device__ __forceinline__ void fetch_sum(const NormArgs<T>& a, size_t base, unsigned off, float (&h)[VEC]) {
-    const Pack<T, VEC> x = fetch<T, VEC, NT>(a.x + base, off);
-    if (a.r) {
-        const Pack<T, VEC> r = fetch<T, VEC, NT>(a.r + base, off);
+// The vectors of one tensor for the K channels of a thread, all on their way before the first is needed (a branch or a
+// conversion in between would wait for each); zeros for a tensor that is not there.
+template <typename T, int VEC, int K, bool NT = false>
+__device__ __forceinline__ void fetch_all(const T* base, const unsigned (&off)[K], Kept<T, VEC> (&v)[K]) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) h[j] = (float)x.v[j] + (float)r.v[j];
-    } else {
+    for (int k = 0; k < K; ++k) v[k] = fetch<T, VEC, NT>(base, off[k]);
+}
+template <typename T, int VEC, int K, bool NT = false>
+__device__ __forceinline__ void fetch_some(const T* t, size_t base, const unsigned (&off)[K], Kept<T, VEC> (&v)[K]) {
+    if (t) fetch_all<T, VEC, K, NT>(t + base, off, v);
+    else {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) h[j] = (float)x.v[j];
+        for (int k = 0; k < K; ++k) v[k] = Pack<T, VEC>{};
+    }
+}
+template <typename T, int VEC, int K>
+__device__ __forceinline__ void add_up(const Kept<T, VEC> (&x)[K], const Kept<T, VEC> (&r)[K], float (&h)[K][VEC]) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const Pack<T, VEC> a = x[k].get(), b = r[k].get();
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) h[k][j] = (float)a.v[j] + (float)b.v[j];
     }
 }
 
@@ -207,7 +231,7 @@ template <typename T, int VEC, bool NT = false> __device__ __forceinline__ void 
 template <int VEC, int LP> struct PlaneTile {
     static constexpr int LC = 64 / LP, TP = LP * VEC;
     int c0, step;                            // first channel of this thread, channel step
-    size_t base, q_base, stride;             // of the map; elements from one of this thread's channels to the next
+    size_t base, q_base;                     // of the map
     unsigned i0;                             // first pixel of this lane's vector
     int fresh;                               // its first pixel that no vector before holds
     template <typename T> __device__ __forceinline__ PlaneTile(const NormArgs<T>& a, unsigned tile) {
@@ -220,10 +244,22 @@ template <int VEC, int LP> struct PlaneTile {
         step = (blockDim.x >> 6) * LC;
         base = (size_t)o * a.C * a.inner;
         q_base = (size_t)o * a.inner;
-        stride = (size_t)step * a.inner;
     }
-    template <typename T> __device__ __forceinline__ unsigned off(const NormArgs<T>& a) const {
-        return ((unsigned)c0 * (unsigned)a.inner + i0) * (unsigned)sizeof(T);
+    // Byte offsets of this thread's channels within the map, and their weights; a channel beyond the last one reads the last one.
+    template <typename T, int K> __device__ __forceinline__ void offsets(const NormArgs<T>& a, unsigned (&off)[K]) const {
+#pragma unroll
+        for (int k = 0; k < K; ++k) off[k] = ((unsigned)min(c0 + k * step, a.C - 1) * (unsigned)a.inner + i0) * (unsigned)sizeof(T);
+    }
+    template <typename T, int K> __device__ __forceinline__ void weights(const NormArgs<T>& a, float (&w)[K]) const {
+#pragma unroll
+        for (int k = 0; k < K; ++k) w[k] = 1.0f;
+        if (a.w && a.w32) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) w[k] = static_cast<const float*>(a.w)[min(c0 + k * step, a.C - 1)];
+        } else if (a.w) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) w[k] = (float)static_cast<const T*>(a.w)[min(c0 + k * step, a.C - 1)];
+        }
     }
 };
 
@@ -254,10 +290,14 @@ template <typename T, int VEC, int LP, int K, bool NT>
 __global__ __launch_bounds__(1024) void k_planes_forward(NormArgs<T> a) {
     __shared__ float lds[16 * LP * VEC];
     const PlaneTile<VEC, LP> t(a, blockIdx.x);
-    const unsigned off = t.off(a);
-    float h[K][VEC], s[VEC] = {};
-#pragma unroll
-    for (int k = 0; k < K; ++k) if (t.c0 + k * t.step < a.C) fetch_sum<T, VEC, NT>(a, t.base + k * t.stride, off, h[k]);
+    unsigned off[K];
+    Kept<T, VEC> x[K], r[K];
+    float h[K][VEC], w[K], s[VEC] = {};
+    t.offsets(a, off);
+    fetch_all<T, VEC, K, NT>(a.x + t.base, off, x);
+    fetch_some<T, VEC, K, NT>(a.r, t.base, off, r);
+    t.weights(a, w);
+    add_up<T, VEC, K>(x, r, h);
 #pragma unroll
     for (int k = 0; k < K; ++k) if (t.c0 + k * t.step < a.C) {
 #pragma unroll
@@ -269,12 +309,11 @@ __global__ __launch_bounds__(1024) void k_planes_forward(NormArgs<T> a) {
     if (t.c0 == 0 && a.q) put<float, VEC>(a.q + t.q_base, t.i0 * 4u, s);
 #pragma unroll
     for (int k = 0; k < K; ++k) if (t.c0 + k * t.step < a.C) {
-        const float w = weight(a, t.c0 + k * t.step);
         float y[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) y[j] = w * (h[k][j] * s[j]);
-        if (a.h) put<T, VEC>(a.h + t.base + k * t.stride, off, h[k]);
-        put<T, VEC>(a.y + t.base + k * t.stride, off, y);
+        for (int j = 0; j < VEC; ++j) y[j] = w[k] * (h[k][j] * s[j]);
+        if (a.h) put<T, VEC>(a.h + t.base, off[k], h[k]);
+        put<T, VEC>(a.y + t.base, off[k], y);
     }
 }
 
@@ -282,47 +321,45 @@ __global__ __launch_bounds__(1024) void k_planes_forward(NormArgs<T> a) {
 template <typename T, int VEC, int LP, int K, bool NT>
 __global__ __launch_bounds__(1024) void k_planes_backward(NormArgs<T> a, unsigned tiles) {
     __shared__ float lds[2][16 * LP * VEC];
-    constexpr bool EARLY = K * VEC <= 16;    // gh on its way with the rest, where the registers allow it
+    constexpr bool EARLY = K * VEC <= 16;    // gh on its way with the rest; where that would spill registers, after the sums
     float dw[K] = {};
     int turn = 0;
     for (unsigned tile = blockIdx.x; tile < tiles; tile += gridDim.x, turn ^= 1) {
         const PlaneTile<VEC, LP> t(a, tile);
-        const unsigned off = t.off(a);
-        float h[K][VEC], g[K][VEC], s[VEC] = {};
-        Pack<T, VEC> gh[K];
-#pragma unroll
-        for (int k = 0; k < K; ++k) if (t.c0 + k * t.step < a.C) {
-            const size_t base = t.base + k * t.stride;
-            fetch_sum<T, VEC, NT>(a, base, off, h[k]);
-            const Pack<T, VEC> p = fetch<T, VEC, NT>(a.gy + base, off);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) g[k][j] = (float)p.v[j];
-            if (EARLY && a.gh) gh[k] = fetch<T, VEC, NT>(a.gh + base, off);
-        }
+        unsigned off[K];
+        Kept<T, VEC> x[K], r[K], g[K], gh[K];
+        float h[K][VEC], w[K], s[VEC] = {};
+        t.offsets(a, off);
+        fetch_all<T, VEC, K, NT>(a.x + t.base, off, x);
+        fetch_some<T, VEC, K, NT>(a.r, t.base, off, r);
+        fetch_all<T, VEC, K, NT>(a.gy + t.base, off, g);
         const Pack<float, VEC> q = fetch<float, VEC>(a.q + t.q_base, t.i0 * 4u);
+        t.weights(a, w);
+        if (EARLY) fetch_some<T, VEC, K, NT>(a.gh, t.base, off, gh);
+        add_up<T, VEC, K>(x, r, h);
 #pragma unroll
-        for (int k = 0; k < K; ++k) if (t.c0 + k * t.step < a.C) {
-            const float w = weight(a, t.c0 + k * t.step);
+        for (int k = 0; k < K; ++k) {
+            const Pack<T, VEC> gy = g[k].get();
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                h[k][j] *= q.v[j];
-                const float gn = g[k][j] * h[k][j];
-                dw[k] += j >= t.fresh ? gn : 0.0f;
-                s[j] = fmaf(w, gn, s[j]);
-                g[k][j] *= w;
+            for (int j = 0; j < VEC; ++j) h[k][j] *= q.v[j];
+            if (t.c0 + k * t.step < a.C) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const float gn = (float)gy.v[j] * h[k][j];
+                    dw[k] += j >= t.fresh ? gn : 0.0f;
+                    s[j] = fmaf(w[k], gn, s[j]);
+                }
             }
         }
         sum_channels<VEC, LP>(s, lds[turn]);
+        if (!EARLY) fetch_some<T, VEC, K, NT>(a.gh, t.base, off, gh);
 #pragma unroll
         for (int k = 0; k < K; ++k) if (t.c0 + k * t.step < a.C) {
+            const Pack<T, VEC> gy = g[k].get(), more = gh[k].get();
             float d[VEC];
-            if (!EARLY && a.gh) gh[k] = fetch<T, VEC, NT>(a.gh + t.base + k * t.stride, off);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                d[j] = q.v[j] * (g[k][j] - h[k][j] * (s[j] * a.inv_c));
-                if (a.gh) d[j] += (float)gh[k].v[j];
-            }
-            put<T, VEC>(a.dx + t.base + k * t.stride, off, d);
+            for (int j = 0; j < VEC; ++j) d[j] = fmaf(q.v[j], (float)gy.v[j] * w[k] - h[k][j] * (s[j] * a.inv_c), (float)more.v[j]);
+            put<T, VEC>(a.dx + t.base, off[k], d);
         }
     }
     if (!a.dw) return;
@@ -361,18 +398,27 @@ template <int G> __device__ __forceinline__ float sum_row(float s, float* lds) {
     return s;
 }
 
-template <typename T, int VEC> __device__ __forceinline__ void weights(const NormArgs<T>& a, int c, float (&w)[VEC]) {
-    if (!a.w) {
+template <typename T, int VEC, int G, int K>
+__device__ __forceinline__ void row_weights(const NormArgs<T>& a, const RowSlot<VEC, G>& t, float (&w)[K][VEC]) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) w[j] = 1.0f;
-    } else if (a.w32) {
-        const Pack<float, VEC> p = fetch<float, VEC>(static_cast<const float*>(a.w), c * 4u);
+    for (int k = 0; k < K; ++k) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) w[j] = p.v[j];
-    } else {
-        const Pack<T, VEC> p = fetch<T, VEC>(static_cast<const T*>(a.w), c * (unsigned)sizeof(T));
+        for (int j = 0; j < VEC; ++j) w[k][j] = 1.0f;
+    }
+    if (a.w && a.w32) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) w[j] = (float)p.v[j];
+        for (int k = 0; k < K; ++k) {
+            const Pack<float, VEC> p = fetch<float, VEC>(static_cast<const float*>(a.w), t.at(k, a.C) * 4u);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) w[k][j] = p.v[j];
+        }
+    } else if (a.w) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const Pack<T, VEC> p = fetch<T, VEC>(static_cast<const T*>(a.w), t.at(k, a.C) * (unsigned)sizeof(T));
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) w[k][j] = (float)p.v[j];
+        }
     }
 }
 
@@ -382,29 +428,33 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void k_rows_forward(NormArgs<T> 
     __shared__ float lds[16];
     const RowSlot<VEC, G> t;
     const size_t row0 = (size_t)blockIdx.x * ROWS, base = row0 * a.C;
-    const unsigned row = threadIdx.x / G;
-    const bool in = row0 + row < a.outer;
-    float h[K][VEC], s = 0.0f;
+    const unsigned rows = (unsigned)min((size_t)ROWS, a.outer - row0), mine = threadIdx.x / G, row = min(mine, rows - 1);
+    unsigned off[K];
+    Kept<T, VEC> x[K], r[K];
+    float h[K][VEC], w[K][VEC], s = 0.0f;
 #pragma unroll
-    for (int k = 0; k < K; ++k) if (in && t.on(k, a.C)) fetch_sum<T, VEC>(a, base, (row * a.C + t.at(k, a.C)) * (unsigned)sizeof(T), h[k]);
+    for (int k = 0; k < K; ++k) off[k] = (row * a.C + t.at(k, a.C)) * (unsigned)sizeof(T);
+    fetch_all<T, VEC, K>(a.x + base, off, x);
+    fetch_some<T, VEC, K>(a.r, base, off, r);
+    row_weights(a, t, w);
+    add_up<T, VEC, K>(x, r, h);
 #pragma unroll
-    for (int k = 0; k < K; ++k) if (in && t.on(k, a.C)) {
+    for (int k = 0; k < K; ++k) if (t.on(k, a.C)) {
         const int fresh = t.fresh(k, a.C);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) s = j >= fresh ? fmaf(h[k][j], h[k][j], s) : s;
     }
     s = sum_row<G>(s, lds);
     const float q = rsqrtf(s * a.inv_c + a.eps);
-    if (in && t.lane == 0 && a.q) a.q[row0 + row] = q;
+    if (mine >= rows) return;
+    if (t.lane == 0 && a.q) a.q[row0 + row] = q;
 #pragma unroll
-    for (int k = 0; k < K; ++k) if (in && t.on(k, a.C)) {
-        const int c = t.at(k, a.C);
-        float w[VEC], y[VEC];
-        weights<T, VEC>(a, c, w);
+    for (int k = 0; k < K; ++k) if (t.on(k, a.C)) {
+        float y[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) y[j] = w[j] * (h[k][j] * q);
-        if (a.h) put<T, VEC>(a.h + base, (row * a.C + c) * (unsigned)sizeof(T), h[k]);
-        put<T, VEC>(a.y + base, (row * a.C + c) * (unsigned)sizeof(T), y);
+        for (int j = 0; j < VEC; ++j) y[j] = w[k][j] * (h[k][j] * q);
+        if (a.h) put<T, VEC>(a.h + base, off[k], h[k]);
+        put<T, VEC>(a.y + base, off[k], y);
     }
 }
 
@@ -414,48 +464,45 @@ __global__ __launch_bounds__(1024) void k_rows_backward(NormArgs<T> a, unsigned 
     constexpr int ROWS = 1024 / G;
     __shared__ float lds[2][16], sum[G * K * VEC];
     const RowSlot<VEC, G> t;
-    const unsigned row = threadIdx.x / G;
-    float dw[K][VEC] = {};
+    const unsigned mine = threadIdx.x / G;
+    float dw[K][VEC] = {}, w[K][VEC];
     int turn = 0;
+    row_weights(a, t, w);
     for (unsigned set = blockIdx.x; set < sets; set += gridDim.x, turn ^= 1) {
         const size_t row0 = (size_t)set * ROWS, base = row0 * a.C;
-        const bool in = row0 + row < a.outer;
-        float h[K][VEC], g[K][VEC], s = 0.0f;
-        Pack<T, VEC> gh[K];
-        const float q = in ? a.q[row0 + row] : 0.0f;
+        const unsigned rows = (unsigned)min((size_t)ROWS, a.outer - row0), row = min(mine, rows - 1);
+        const bool in = mine < rows;
+        unsigned off[K];
+        Kept<T, VEC> x[K], r[K], g[K], gh[K];
+        float h[K][VEC], s = 0.0f;
 #pragma unroll
-        for (int k = 0; k < K; ++k) if (in && t.on(k, a.C)) {
-            const unsigned off = (row * a.C + t.at(k, a.C)) * (unsigned)sizeof(T);
-            fetch_sum<T, VEC>(a, base, off, h[k]);
-            const Pack<T, VEC> p = fetch<T, VEC>(a.gy + base, off);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) g[k][j] = (float)p.v[j];
-            if (a.gh) gh[k] = fetch<T, VEC>(a.gh + base, off);
-        }
+        for (int k = 0; k < K; ++k) off[k] = (row * a.C + t.at(k, a.C)) * (unsigned)sizeof(T);
+        fetch_all<T, VEC, K>(a.x + base, off, x);
+        fetch_some<T, VEC, K>(a.r, base, off, r);
+        fetch_all<T, VEC, K>(a.gy + base, off, g);
+        const float q = a.q[row0 + row];
+        fetch_some<T, VEC, K>(a.gh, base, off, gh);
+        add_up<T, VEC, K>(x, r, h);
 #pragma unroll
         for (int k = 0; k < K; ++k) if (in && t.on(k, a.C)) {
             const int fresh = t.fresh(k, a.C);
-            float w[VEC];
-            weights<T, VEC>(a, t.at(k, a.C), w);
+            const Pack<T, VEC> gy = g[k].get();
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
                 h[k][j] *= q;
-                const float gn = g[k][j] * h[k][j];
+                const float gn = (float)gy.v[j] * h[k][j];
                 dw[k][j] += gn;
-                g[k][j] *= w[j];
-                s = j >= fresh ? fmaf(w[j], gn, s) : s;
+                s = j >= fresh ? fmaf(w[k][j], gn, s) : s;
             }
         }
         s = sum_row<G>(s, lds[turn]) * a.inv_c;
 #pragma unroll
         for (int k = 0; k < K; ++k) if (in && t.on(k, a.C)) {
+            const Pack<T, VEC> gy = g[k].get(), more = gh[k].get();
             float d[VEC];
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                d[j] = q * (g[k][j] - h[k][j] * s);
-                if (a.gh) d[j] += (float)gh[k].v[j];
-            }
-            put<T, VEC>(a.dx + base, (row * a.C + t.at(k, a.C)) * (unsigned)sizeof(T), d);
+            for (int j = 0; j < VEC; ++j) d[j] = fmaf(q, (float)gy.v[j] * w[k][j] - h[k][j] * s, (float)more.v[j]);
+            put<T, VEC>(a.dx + base, off[k], d);
         }
     }
     if (!a.dw) return;
@@ -469,10 +516,10 @@ __global__ __launch_bounds__(1024) void k_rows_backward(NormArgs<T> a, unsigned 
         }
     }
     constexpr int TURNS = G < 64 ? 16 : ROWS;
-    const int mine = G < 64 ? threadIdx.x >> 6 : threadIdx.x / G;
+    const int my_turn = G < 64 ? threadIdx.x >> 6 : threadIdx.x / G;
     const bool first = G >= 64 || (threadIdx.x & 63) < G;
     for (int r = 0; r < TURNS; ++r) {
-        if (r == mine && first) {
+        if (r == my_turn && first) {
 #pragma unroll
             for (int k = 0; k < K; ++k) {
 #pragma unroll
