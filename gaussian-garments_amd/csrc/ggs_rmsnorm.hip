@@ -164,9 +164,9 @@ typedef unsigned Bits16 __attribute__((ext_vector_type(4), aligned(2)));
 // NT: past the caches (see STREAM_BYTES)
 template <typename T, int VEC, bool NT = false> __device__ __forceinline__ Pack<T, VEC> fetch(const T* base, unsigned off) {
     const char* at = reinterpret_cast<const char*>(base) + off;
-    if constexpr (NT) {
-        static_assert(sizeof(Pack<T, VEC>) == 16, "one 16-byte access");
-        const Bits16 v = __builtin_nontemporal_load(reinterpret_cast<const Bits16*>(at));
+    if constexpr (sizeof(Pack<T, VEC>) == 16) {
+        const Bits16* p = reinterpret_cast<const Bits16*>(at);
+        const Bits16 v = NT ? __builtin_nontemporal_load(p) : *p;
         Pack<T, VEC> o;
         __builtin_memcpy(&o, &v, 16);
         return o;
@@ -177,11 +177,14 @@ template <typename T, int VEC, bool NT = false> __device__ __forceinline__ Pack<
 // A pack that stays in registers between phases: as four words, where the compiler would give every 16-bit element one
 template <typename T, int VEC, bool WIDE = sizeof(T) * VEC == 16> struct Kept {
     Bits16 b;
+    // an unpacked copy does not outlive this point
+    __device__ __forceinline__ void pin() { asm volatile("" : "+v"(b[0]), "+v"(b[1]), "+v"(b[2]), "+v"(b[3])); }
     __device__ __forceinline__ void operator=(const Pack<T, VEC>& p) { __builtin_memcpy(&b, &p, 16); }
     __device__ __forceinline__ Pack<T, VEC> get() const { Pack<T, VEC> p; __builtin_memcpy(&p, &b, 16); return p; }
 };
 template <typename T, int VEC> struct Kept<T, VEC, false> {
     Pack<T, VEC> p;
+    __device__ __forceinline__ void pin() {}
     __device__ __forceinline__ void operator=(const Pack<T, VEC>& o) { p = o; }
     __device__ __forceinline__ Pack<T, VEC> get() const { return p; }
 };
@@ -245,20 +248,22 @@ template <int VEC, int LP> struct PlaneTile {
         base = (size_t)o * a.C * a.inner;
         q_base = (size_t)o * a.inner;
     }
-    // Byte offsets of this thread's channels within the map, and their weights; a channel beyond the last one reads the last one.
+    // Byte offsets of this thread's channels within the map; a channel beyond the last one reads the last one.
     template <typename T, int K> __device__ __forceinline__ void offsets(const NormArgs<T>& a, unsigned (&off)[K]) const {
 #pragma unroll
         for (int k = 0; k < K; ++k) off[k] = ((unsigned)min(c0 + k * step, a.C - 1) * (unsigned)a.inner + i0) * (unsigned)sizeof(T);
     }
-    template <typename T, int K> __device__ __forceinline__ void weights(const NormArgs<T>& a, float (&w)[K]) const {
+    // Their weights, the same for every tile.
+    template <typename T, int K> static __device__ __forceinline__ void weights(const NormArgs<T>& a, float (&w)[K]) {
+        const unsigned c0 = (threadIdx.x >> 6) * LC + (threadIdx.x & 63) / LP, step = (blockDim.x >> 6) * LC, last = a.C - 1;
 #pragma unroll
         for (int k = 0; k < K; ++k) w[k] = 1.0f;
         if (a.w && a.w32) {
 #pragma unroll
-            for (int k = 0; k < K; ++k) w[k] = static_cast<const float*>(a.w)[min(c0 + k * step, a.C - 1)];
+            for (int k = 0; k < K; ++k) w[k] = static_cast<const float*>(a.w)[min(c0 + k * step, last)];
         } else if (a.w) {
 #pragma unroll
-            for (int k = 0; k < K; ++k) w[k] = (float)static_cast<const T*>(a.w)[min(c0 + k * step, a.C - 1)];
+            for (int k = 0; k < K; ++k) w[k] = (float)static_cast<const T*>(a.w)[min(c0 + k * step, last)];
         }
     }
 };
@@ -322,19 +327,19 @@ template <typename T, int VEC, int LP, int K, bool NT>
 __global__ __launch_bounds__(1024) void k_planes_backward(NormArgs<T> a, unsigned tiles) {
     __shared__ float lds[2][16 * LP * VEC];
     constexpr bool EARLY = K * VEC <= 16;    // gh on its way with the rest; where that would spill registers, after the sums
-    float dw[K] = {};
+    float dw[K] = {}, w[K];
     int turn = 0;
+    PlaneTile<VEC, LP>::weights(a, w);
     for (unsigned tile = blockIdx.x; tile < tiles; tile += gridDim.x, turn ^= 1) {
         const PlaneTile<VEC, LP> t(a, tile);
         unsigned off[K];
         Kept<T, VEC> x[K], r[K], g[K], gh[K];
-        float h[K][VEC], w[K], s[VEC] = {};
+        float h[K][VEC], s[VEC] = {};
         t.offsets(a, off);
         fetch_all<T, VEC, K, NT>(a.x + t.base, off, x);
         fetch_some<T, VEC, K, NT>(a.r, t.base, off, r);
         fetch_all<T, VEC, K, NT>(a.gy + t.base, off, g);
         const Pack<float, VEC> q = fetch<float, VEC>(a.q + t.q_base, t.i0 * 4u);
-        t.weights(a, w);
         if (EARLY) fetch_some<T, VEC, K, NT>(a.gh, t.base, off, gh);
         add_up<T, VEC, K>(x, r, h);
 #pragma unroll
@@ -352,7 +357,11 @@ __global__ __launch_bounds__(1024) void k_planes_backward(NormArgs<T> a, unsigne
             }
         }
         sum_channels<VEC, LP>(s, lds[turn]);
-        if (!EARLY) fetch_some<T, VEC, K, NT>(a.gh, t.base, off, gh);
+        if (!EARLY) {
+            fetch_some<T, VEC, K, NT>(a.gh, t.base, off, gh);
+#pragma unroll
+            for (int k = 0; k < K; ++k) g[k].pin();
+        }
 #pragma unroll
         for (int k = 0; k < K; ++k) if (t.c0 + k * t.step < a.C) {
             const Pack<T, VEC> gy = g[k].get(), more = gh[k].get();
