@@ -471,6 +471,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void k_rows_forward(NormArgs<T> 
 template <typename T, int VEC, int G, int K>
 __global__ __launch_bounds__(1024) void k_rows_backward(NormArgs<T> a, unsigned sets) {
     constexpr int ROWS = 1024 / G;
+    constexpr bool EARLY = K * VEC <= 16 && K < 4;       // gh: as in k_planes_backward
     __shared__ float lds[2][16], sum[G * K * VEC];
     const RowSlot<VEC, G> t;
     const unsigned mine = threadIdx.x / G;
@@ -490,7 +491,7 @@ __global__ __launch_bounds__(1024) void k_rows_backward(NormArgs<T> a, unsigned 
         fetch_some<T, VEC, K>(a.r, base, off, r);
         fetch_all<T, VEC, K>(a.gy + base, off, g);
         const float q = a.q[row0 + row];
-        fetch_some<T, VEC, K>(a.gh, base, off, gh);
+        if (EARLY) fetch_some<T, VEC, K>(a.gh, base, off, gh);
         add_up<T, VEC, K>(x, r, h);
 #pragma unroll
         for (int k = 0; k < K; ++k) if (in && t.on(k, a.C)) {
@@ -505,6 +506,11 @@ __global__ __launch_bounds__(1024) void k_rows_backward(NormArgs<T> a, unsigned 
             }
         }
         s = sum_row<G>(s, lds[turn]) * a.inv_c;
+        if (!EARLY) {
+            fetch_some<T, VEC, K>(a.gh, base, off, gh);
+#pragma unroll
+            for (int k = 0; k < K; ++k) g[k].pin();
+        }
 #pragma unroll
         for (int k = 0; k < K; ++k) if (in && t.on(k, a.C)) {
             const Pack<T, VEC> gy = g[k].get(), more = gh[k].get();
@@ -550,7 +556,7 @@ __global__ __launch_bounds__(1024) void k_rows_backward(NormArgs<T> a, unsigned 
 
 // ---- which kernel ----------------------------------------------------------------------------------------------------------
 // One-pass kernels: float and 16-bit types, a pixel's channels within the registers of one workgroup (1024 channels of a map,
-// 2048 vectors of a row), a map within 32-bit offsets; the two-pass kernels serve double and what is left.
+// 16384 of a row), a map within 32-bit offsets; the two-pass kernels serve double and what is left.
 struct Plan {
     int kind;                    // 0 two passes, 1 planes, 2 rows
     int vec, lanes, k, waves;    // planes: LP and waves of a workgroup; rows: G
@@ -568,8 +574,8 @@ template <typename T> Plan plan(size_t outer, int C, size_t inner) {
         const int vec = C >= FULL ? FULL : 1, vecs = (C + vec - 1) / vec;
         const int lanes = vecs <= 8 ? 4 : vecs <= 32 ? 16 : vecs <= 128 ? 64 : vecs <= 512 ? 256 : 1024;
         const size_t sets = (outer + 1024 / lanes - 1) / (1024 / lanes);
-        if (vecs > 2048 || sets > 0x7fffffffu / 4) return p;          // (the forward kernel's workgroups take a quarter of a set)
-        p.kind = 2; p.vec = vec; p.lanes = lanes; p.k = vecs <= lanes ? 1 : 2; p.tiles = sets;
+        if (vecs > (sizeof(T) == 4 ? 4096 : 2048) || sets > 0x7fffffffu / 4) return p;          // (the forward kernel's workgroups take a quarter of a set)
+        p.kind = 2; p.vec = vec; p.lanes = lanes; p.k = vecs <= lanes ? 1 : vecs <= 2 * lanes ? 2 : 4; p.tiles = sets;
         p.partials = (int)(sets < 256 ? sets : 256);
         return p;
     }
@@ -626,7 +632,8 @@ template <typename T> void one_pass(bool back, const NormArgs<T>& a, const Plan&
         else if (p.lanes == 16) rows<T, FULL, 16>(back, a, p, s);
         else if (p.lanes == 64) rows<T, FULL, 64>(back, a, p, s);
         else if (p.lanes == 256) rows<T, FULL, 256>(back, a, p, s);
-        else rows<T, FULL, 1024>(back, a, p, s);
+        else if (p.k < 4) rows<T, FULL, 1024>(back, a, p, s);
+        else if constexpr (sizeof(T) == 4) rows<T, FULL, 1024, 4>(back, a, p, s);
         return;
     }
     if (p.vec == 1) planes<T, 1, 4>(back, a, p, s);
