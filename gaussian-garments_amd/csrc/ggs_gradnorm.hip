@@ -16,7 +16,7 @@
 namespace {
 
 #define GGS_NORM_MAX_TENSORS 128          // gradients per launch: a table of 2.7 KB in the kernel arguments
-#define GGS_NORM_MAX_BLOCKS 512           // partial sums per launch
+#define GGS_NORM_MAX_BLOCKS 1024          // partial sums per launch
 #define GGS_NORM_CHUNK 1024               // 16-byte vectors of one tensor a workgroup takes at a time
 
 struct GradTable {
@@ -39,30 +39,30 @@ __device__ __forceinline__ double block_sum(double s) {
     return (part[0] + part[1]) + (part[2] + part[3]);
 }
 
-// Calls f(pack, vector of the tensor, whole) for the vectors of one chunk; a pack that reaches over either end of the tensor
-// is filled element by element (zeros outside).  The 16-byte grid is the address space's: a gradient that is a view into a
-// flat bucket starts anywhere.
+// Calls f(packs, store) for a chunk, four packs a thread: all of them on their way before the first is needed where the whole
+// chunk lies inside the tensor; otherwise packs that reach over either end are filled element by element (zeros outside).  The
+// 16-byte grid is the address space's: a gradient that is a view into a flat bucket starts anywhere.
 template <typename T, typename F>
 __device__ __forceinline__ void for_chunk(void* ptr, size_t numel, unsigned chunk, F&& f) {
     constexpr int VEC = 16 / sizeof(T);
     const unsigned shift = (unsigned)((reinterpret_cast<uintptr_t>(ptr) & 15) / sizeof(T));
     T* base = static_cast<T*>(ptr) - shift;
-    const size_t nv = (numel + shift + VEC - 1) / VEC, v0 = (size_t)chunk * GGS_NORM_CHUNK + threadIdx.x;
-    const size_t end = numel + shift;
+    const size_t end = numel + shift, c0 = (size_t)chunk * GGS_NORM_CHUNK;
+    Pack16<T> p[4];
+    if ((c0 > 0 || shift == 0) && (c0 + GGS_NORM_CHUNK) * VEC <= end) {
+        Pack16<T>* at = reinterpret_cast<Pack16<T>*>(base) + c0 + threadIdx.x;
 #pragma unroll
-    for (int k = 0; k < GGS_NORM_CHUNK / 256; ++k) {
-        const size_t v = v0 + k * 256;
-        if (v >= nv) break;
-        if ((v > 0 || shift == 0) && (v + 1) * VEC <= end) {
-            Pack16<T>* at = reinterpret_cast<Pack16<T>*>(base) + v;
-            f(*at, [&](const Pack16<T>& p) { *at = p; });
-        } else {
-            Pack16<T> p;
-            for (int j = 0; j < VEC; ++j) p.v[j] = v * VEC + j >= shift && v * VEC + j < end ? base[v * VEC + j] : (T)0.0f;
-            f(p, [&](const Pack16<T>& q) {
-                for (int j = 0; j < VEC; ++j) if (v * VEC + j >= shift && v * VEC + j < end) base[v * VEC + j] = q.v[j];
-            });
+        for (int k = 0; k < 4; ++k) p[k] = at[k * 256];
+        f(p, [&](int k, const Pack16<T>& q) { at[k * 256] = q; });
+    } else {
+        for (int k = 0; k < 4; ++k) {
+            const size_t e = (c0 + threadIdx.x + k * 256) * VEC;
+            for (int j = 0; j < VEC; ++j) p[k].v[j] = e + j >= shift && e + j < end ? base[e + j] : (T)0.0f;
         }
+        f(p, [&](int k, const Pack16<T>& q) {
+            const size_t e = (c0 + threadIdx.x + k * 256) * VEC;
+            for (int j = 0; j < VEC; ++j) if (e + j >= shift && e + j < end) base[e + j] = q.v[j];
+        });
     }
 }
 
@@ -77,12 +77,15 @@ struct Finder {
 
 template <typename T>
 __device__ __forceinline__ double chunk_squares(void* g, size_t numel, unsigned chunk) {
-    double s = 0.0;
-    for_chunk<T>(g, numel, chunk, [&](const Pack16<T>& p, auto&&) {
+    double s[4] = {};
+    for_chunk<T>(g, numel, chunk, [&](const Pack16<T> (&p)[4], auto&&) {
 #pragma unroll
-        for (int j = 0; j < (int)(16 / sizeof(T)); ++j) { const double d = (double)(float)p.v[j]; s = fma(d, d, s); }
+        for (int k = 0; k < 4; ++k) {
+#pragma unroll
+            for (int j = 0; j < (int)(16 / sizeof(T)); ++j) { const double d = (double)(float)p[k].v[j]; s[k] = fma(d, d, s[k]); }
+        }
     });
-    return s;
+    return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
 __global__ __launch_bounds__(256) void k_grad_squares(GradTable t, double* partial) {
@@ -122,10 +125,13 @@ __global__ __launch_bounds__(256) void k_grad_norm(const double* partial, int n,
 
 template <typename T>
 __device__ __forceinline__ void chunk_scale(void* g, size_t numel, unsigned chunk, float c) {
-    for_chunk<T>(g, numel, chunk, [&](Pack16<T> p, auto&& store) {
+    for_chunk<T>(g, numel, chunk, [&](Pack16<T> (&p)[4], auto&& store) {
 #pragma unroll
-        for (int j = 0; j < (int)(16 / sizeof(T)); ++j) p.v[j] = (T)((float)p.v[j] * c);
-        store(p);
+        for (int k = 0; k < 4; ++k) {
+#pragma unroll
+            for (int j = 0; j < (int)(16 / sizeof(T)); ++j) p[k].v[j] = (T)((float)p[k].v[j] * c);
+            store(k, p[k]);
+        }
     });
 }
 
@@ -148,7 +154,8 @@ __global__ __launch_bounds__(256) void k_grad_scale(GradTable t, const double* p
 }
 
 // ---- the clipped update ---------------------------------------------------------------------------------------------------
-#define GGS_CLIP_MAX_TENSORS 48
+#define GGS_CLIP_MAX_TENSORS 64           // a table of 3.9 KB
+#define GGS_CLIP_BLOCKS 2048              // workgroups a launch, about
 struct ClipAdam {
     int n, tick;
     unsigned first_block[GGS_CLIP_MAX_TENSORS + 1];
@@ -170,13 +177,22 @@ __device__ __forceinline__ void adam1(float& p, float g, float& m, float& v, con
     p = fmaf(-step_size, m / (sqrtf(v) / bias2_sqrt + a.eps), p);
 }
 
+struct AdamVec { float4 p, g, m, v; };
+
 __global__ __launch_bounds__(256) void k_adam_clip(ClipAdam a) {
     if (a.guard && *a.guard) return;
-    const double d = norm_of(a.partial, a.n_partial);
-    if (a.norm && blockIdx.x == 0 && threadIdx.x == 0) *a.norm = (float)d;
-    const float f = clip_factor(d, a.max_norm);
-    int t = 0;
-    while (t + 1 < a.n && blockIdx.x >= a.first_block[t + 1]) ++t;
+    const int l = threadIdx.x & 63;
+    const unsigned end_block = l < a.n ? a.first_block[l + 1] : ~0u;
+    const int t = __builtin_amdgcn_readfirstlane((int)__popcll(__ballot(end_block <= blockIdx.x)));
+    const unsigned b0 = a.first_block[t], nb = a.first_block[t + 1] - b0;
+    const size_t n = a.numel[t], n4 = n / 4, stride = (size_t)nb * 256;
+    float4* p4 = reinterpret_cast<float4*>(a.p[t]);
+    const float4* g4 = reinterpret_cast<const float4*>(a.g[t]);
+    float4* m4 = reinterpret_cast<float4*>(a.m[t]);
+    float4* v4 = reinterpret_cast<float4*>(a.v[t]);
+    size_t i = (size_t)(blockIdx.x - b0) * 256 + threadIdx.x;
+    AdamVec now, next;                       // one iteration ahead: the first loads run beside the sum of the partials
+    if (i < n4) now = {p4[i], g4[i], m4[i], v4[i]};
     AdamState* st = a.s[t];
     float bias1 = st->bias1, bs = st->bias2_sqrt;
     long long tt = 0;
@@ -189,24 +205,21 @@ __global__ __launch_bounds__(256) void k_adam_clip(ClipAdam a) {
         bs = (float)sqrt(1.0 - p2);
     }
     const float step_size = *a.lr[t] / bias1;
-    const unsigned b0 = a.first_block[t], nb = a.first_block[t + 1] - b0;
-    const size_t n = a.numel[t], n4 = n / 4, stride = (size_t)nb * 256;
-    float4* p4 = reinterpret_cast<float4*>(a.p[t]);
-    const float4* g4 = reinterpret_cast<const float4*>(a.g[t]);
-    float4* m4 = reinterpret_cast<float4*>(a.m[t]);
-    float4* v4 = reinterpret_cast<float4*>(a.v[t]);
-    for (size_t i = (size_t)(blockIdx.x - b0) * 256 + threadIdx.x; i < n4; i += stride) {
-        float4 p = p4[i], m = m4[i], v = v4[i];
-        const float4 g = g4[i];
-        adam1(p.x, g.x * f, m.x, v.x, a, step_size, bs);
-        adam1(p.y, g.y * f, m.y, v.y, a, step_size, bs);
-        adam1(p.z, g.z * f, m.z, v.z, a, step_size, bs);
-        adam1(p.w, g.w * f, m.w, v.w, a, step_size, bs);
-        p4[i] = p; m4[i] = m; v4[i] = v;
+    const double d = norm_of(a.partial, a.n_partial);
+    if (a.norm && blockIdx.x == 0 && threadIdx.x == 0) *a.norm = (float)d;
+    const float f = clip_factor(d, a.max_norm);
+    for (; i < n4; i += stride, now = next) {
+        const size_t j = i + stride;
+        if (j < n4) next = {p4[j], g4[j], m4[j], v4[j]};
+        adam1(now.p.x, now.g.x * f, now.m.x, now.v.x, a, step_size, bs);
+        adam1(now.p.y, now.g.y * f, now.m.y, now.v.y, a, step_size, bs);
+        adam1(now.p.z, now.g.z * f, now.m.z, now.v.z, a, step_size, bs);
+        adam1(now.p.w, now.g.w * f, now.m.w, now.v.w, a, step_size, bs);
+        p4[i] = now.p; m4[i] = now.m; v4[i] = now.v;
     }
     if (blockIdx.x == b0 && threadIdx.x < (n & 3)) {
-        const size_t i = n4 * 4 + threadIdx.x;
-        adam1(a.p[t][i], a.g[t][i] * f, a.m[t][i], a.v[t][i], a, step_size, bs);
+        const size_t k = n4 * 4 + threadIdx.x;
+        adam1(a.p[t][k], a.g[t][k] * f, a.m[t][k], a.v[t][k], a, step_size, bs);
     }
     if (a.tick) __syncthreads();             // every wave of this workgroup has read the state (its values fed the loop above)
     if (a.tick && threadIdx.x == 0) {        // as in ggs_adam.hip: the last workgroup of a tensor stores the advanced state
@@ -350,15 +363,21 @@ int ggs_adam_clip_step(int n_tensors, const size_t* numel, float* const* params,
     a.beta2 = (float)beta2; a.omb1 = (float)(1.0 - beta1); a.omb2 = (float)(1.0 - beta2); a.eps = (float)eps;
     a.beta1d = beta1; a.beta2d = beta2;
     for (int i = 0; i < n_tensors;) {
+        int end = i;                                              // the tensors of this launch
+        size_t total = 0;
+        for (int k = 0; end < n_tensors && k < GGS_CLIP_MAX_TENSORS; ++end) {
+            k += numel[end] != 0;
+            total += numel[end];
+        }
+        // vectors a workgroup takes: enough of them that adding up the partials is a small part of its work
+        const size_t share = total / 4 / GGS_CLIP_BLOCKS < 256 ? 256 : total / 4 / GGS_CLIP_BLOCKS;
         a.n = 0; a.first_block[0] = 0;
-        for (; i < n_tensors && a.n < GGS_CLIP_MAX_TENSORS; ++i) {
+        for (; i < end; ++i) {
             if (numel[i] == 0) continue;
             const int k = a.n++;
             a.numel[k] = numel[i]; a.p[k] = params[i]; a.g[k] = grads[i]; a.m[k] = exp_avgs[i]; a.v[k] = exp_avg_sqs[i];
             a.lr[k] = lrs[i]; a.s[k] = static_cast<AdamState*>(states[i]);
-            size_t blocks = (numel[i] / 4 + 255) / 256;
-            blocks = blocks < 1 ? 1 : (blocks > 1024 ? 1024 : blocks);
-            a.first_block[k + 1] = a.first_block[k] + (unsigned)blocks;
+            a.first_block[k + 1] = a.first_block[k] + (unsigned)(numel[i] / 4 < share ? 1 : (numel[i] / 4 + share - 1) / share);
         }
         if (a.n == 0) break;
         hipLaunchKernelGGL(k_adam_clip, dim3(a.first_block[a.n]), dim3(256), 0, s, a);
