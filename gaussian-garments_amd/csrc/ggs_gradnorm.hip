@@ -177,6 +177,17 @@ __device__ __forceinline__ void adam1(float& p, float g, float& m, float& v, con
     p = fmaf(-step_size, m / (sqrtf(v) / bias2_sqrt + a.eps), p);
 }
 
+// Parameters and moments pass by the caches in both directions: they come back a step later, and what they would push out is the
+// gradient the norm has just read (43.8M parameters, norm and update: 309 -> 280 us; 6M: 50.0 -> 48.7 us).
+typedef float Float4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ float4 load_past(const float4* p) {
+    const Float4 v = __builtin_nontemporal_load(reinterpret_cast<const Float4*>(p));
+    return make_float4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ void store_past(float4* p, const float4& a) {
+    const Float4 v = {a.x, a.y, a.z, a.w};
+    __builtin_nontemporal_store(v, reinterpret_cast<Float4*>(p));
+}
 struct AdamVec { float4 p, g, m, v; };
 
 __global__ __launch_bounds__(256) void k_adam_clip(ClipAdam a) {
@@ -192,7 +203,7 @@ __global__ __launch_bounds__(256) void k_adam_clip(ClipAdam a) {
     float4* v4 = reinterpret_cast<float4*>(a.v[t]);
     size_t i = (size_t)(blockIdx.x - b0) * 256 + threadIdx.x;
     AdamVec now, next;                       // one iteration ahead: the first loads run beside the sum of the partials
-    if (i < n4) now = {p4[i], g4[i], m4[i], v4[i]};
+    if (i < n4) now = {load_past(p4 + i), g4[i], load_past(m4 + i), load_past(v4 + i)};
     AdamState* st = a.s[t];
     float bias1 = st->bias1, bs = st->bias2_sqrt;
     long long tt = 0;
@@ -210,12 +221,12 @@ __global__ __launch_bounds__(256) void k_adam_clip(ClipAdam a) {
     const float f = clip_factor(d, a.max_norm);
     for (; i < n4; i += stride, now = next) {
         const size_t j = i + stride;
-        if (j < n4) next = {p4[j], g4[j], m4[j], v4[j]};
+        if (j < n4) next = {load_past(p4 + j), g4[j], load_past(m4 + j), load_past(v4 + j)};
         adam1(now.p.x, now.g.x * f, now.m.x, now.v.x, a, step_size, bs);
         adam1(now.p.y, now.g.y * f, now.m.y, now.v.y, a, step_size, bs);
         adam1(now.p.z, now.g.z * f, now.m.z, now.v.z, a, step_size, bs);
         adam1(now.p.w, now.g.w * f, now.m.w, now.v.w, a, step_size, bs);
-        p4[i] = now.p; m4[i] = now.m; v4[i] = now.v;
+        store_past(p4 + i, now.p); store_past(m4 + i, now.m); store_past(v4 + i, now.v);
     }
     if (blockIdx.x == b0 && threadIdx.x < (n & 3)) {
         const size_t k = n4 * 4 + threadIdx.x;
