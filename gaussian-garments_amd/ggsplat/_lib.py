@@ -225,14 +225,3 @@ def dtype_code(dt) -> int:
         return {torch.float32: 0, torch.float16: 1, torch.float64: 2}[dt]
     except KeyError:
         raise RuntimeError(f'"ggsplat stylegan op" not implemented for \'{str(dt).replace("torch.", "")}\'') from None
-
-
-_NORM_DTYPES = {torch.float32: 0, torch.float16: 1, torch.float64: 2, torch.bfloat16: 3}
-
-
-def norm_dtype_code(dt, allowed=tuple(_NORM_DTYPES)) -> int:
-    """GGS_DTYPE_* for the entry points that also take bfloat16 (ggs_rms_norm_*, ggs_grad_*)."""
-    if dt not in allowed:
-        raise TypeError(f"ggsplat: {str(dt).replace('torch.', '')} is not one of "
-                        + ", ".join(str(d).replace("torch.", "") for d in allowed))
-    return _NORM_DTYPES[dt]

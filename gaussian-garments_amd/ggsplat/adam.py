@@ -23,9 +23,7 @@ from typing import Dict, Iterable, List, Optional
 
 import torch
 
-from ._lib import check, lib, norm_dtype_code, on_device, ptr, stream_ptr
-
-_GRAD_TYPES = (torch.float32, torch.float16, torch.bfloat16)
+from ._lib import check, lib, on_device, ptr, stream_ptr
 
 
 def _checked_max_norm(max_norm) -> float:
@@ -46,50 +44,65 @@ def _span(t: torch.Tensor):
     return span, dense, shared
 
 
+_GRAD_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 3}              # GGS_DTYPE_*
+_GRAD_SIZE = {0: 4, 1: 2, 3: 2}
+
+
 class _GradList:
     """The gradients of one call as the C ABI takes them: sizes, addresses, types.  The order of a tensor's elements is of no
     matter to the norm, so any dense layout is read in place; a strided one is read (and written back) through a copy."""
 
     def __init__(self, grads, in_place: bool):
-        grads = [grads] if isinstance(grads, torch.Tensor) else [g for g in grads if g is not None]
-        self.device, self.copies, spans, kept = None, [], [], []
-        for g in grads:
+        self.device, self.copies, self.keep = None, [], []
+        index, numel, ptrs, types, ends = None, [], [], [], []
+        for g in ([grads] if isinstance(grads, torch.Tensor) else grads):
+            if g is None:
+                continue
             if not isinstance(g, torch.Tensor):
                 raise TypeError(f"ggsplat: gradients are tensors, got {type(g).__name__}")
-            if g.device.type != "cuda":
+            at = g.get_device()
+            if at < 0:
                 raise RuntimeError("ggsplat: gradient norms run on the GPU only (no CPU path in the product)")
             if g.requires_grad:
                 raise ValueError("ggsplat: pass the gradients ([p.grad for p in params]), not the parameters")
-            if g.layout != torch.strided:
+            if g.layout is not torch.strided:
                 raise TypeError("ggsplat: sparse gradients are not supported")
-            if self.device is None:
-                self.device = g.device
-            elif g.device != self.device:
-                raise ValueError("ggsplat: the gradients are on different devices")
-            code = norm_dtype_code(g.dtype, _GRAD_TYPES)
+            if at != index:
+                if index is not None:
+                    raise ValueError("ggsplat: the gradients are on different devices")
+                index, self.device = at, g.device
+            code = _GRAD_CODES.get(g.dtype)
+            if code is None:
+                raise TypeError(f"ggsplat: gradients are float32, float16 or bfloat16, got {g.dtype}")
             n = g.numel()
             if n == 0:
                 continue
-            span, dense, shared = (n, True, False) if g.is_contiguous() else _span(g)
-            if in_place:
-                if shared:
+            span = n
+            if not g.is_contiguous():
+                span, dense, shared = _span(g)
+                if in_place and shared:
                     raise ValueError("ggsplat: a gradient's elements share memory (an expanded tensor?): make it contiguous first")
-                at = g.data_ptr()
-                spans.append((at, at + span * g.element_size()))
-            if not dense:
-                c = g.contiguous()
-                self.copies.append((g, c))
-                g = c
-            kept.append((n, g.data_ptr(), code, g))
-        if in_place:
-            spans.sort()
-            if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
-                raise ValueError("ggsplat: two of the gradients overlap in memory (the same one listed twice?)")
-        self.n = n = len(kept)
-        self.keep = [k[3] for k in kept]
-        self.numel = (C.c_size_t * n)(*[k[0] for k in kept])
-        self.ptrs = (C.c_void_p * n)(*[k[1] for k in kept])
-        self.types = (C.c_int * n)(*[k[2] for k in kept])
+                if in_place:
+                    ends.append((g.data_ptr(), g.data_ptr() + span * _GRAD_SIZE[code]))
+                if not dense:
+                    c = g.contiguous()
+                    self.copies.append((g, c))
+                    g = c
+            elif in_place:
+                ends.append((g.data_ptr(), g.data_ptr() + n * _GRAD_SIZE[code]))
+            self.keep.append(g)
+            numel.append(n)
+            ptrs.append(g.data_ptr())
+            types.append(code)
+        if in_place and len(ends) > 1:
+            ends.sort()
+            last = 0
+            for lo, hi in ends:
+                if lo < last:
+                    raise ValueError("ggsplat: two of the gradients overlap in memory (the same one listed twice?)")
+                last = hi
+        self.n = n = len(numel)
+        self.numel, self.ptrs, self.types = (C.c_size_t * n)(*numel), (C.c_void_p * n)(*ptrs), (C.c_int * n)(*types)
 
     def buffers(self):
         """(the norm, workspace bytes, workspace): new for every call, so that calls on several streams and captured graphs
@@ -286,36 +299,49 @@ class GraphAdam:
             raise ValueError("GraphAdam.step: guard must be a 64-bit word on the optimiser's device")
         gp = ptr(guard)
         b1, b2 = self.betas
-        # every tensor that has a gradient: one launch per 16 tensors
-        items = []
-        for i, g in enumerate(self.param_groups):
+        # every tensor that has a gradient: sizes, the six columns of addresses, and the gradients themselves (copies live on)
+        numel, cols, keep, f32 = [], ([], [], [], [], [], []), [], torch.float32
+        add_p, add_g, add_m, add_v, add_lr, add_s = (c.append for c in cols)
+        states, lr = self.state, self._lr_dev.data_ptr()
+        for g in self.param_groups:
             for p in g["params"]:
-                if p.grad is None or p.numel() == 0:
+                grad = p.grad
+                if grad is None:
                     continue
-                grad = p.grad if (p.grad.is_contiguous() and p.grad.dtype == torch.float32) else p.grad.float().contiguous()
-                st = self.state[p]
-                items.append((p.numel(), p.data_ptr(), grad.data_ptr(), st["exp_avg"].data_ptr(),
-                              st["exp_avg_sq"].data_ptr(), self._lr_dev.data_ptr() + 4 * i, st["state"].data_ptr(), grad))
+                n = p.numel()
+                if n == 0:
+                    continue
+                if grad.dtype is not f32 or not grad.is_contiguous():
+                    grad = grad.float().contiguous()
+                st = states[p]
+                numel.append(n)
+                keep.append(grad)
+                add_p(p.data_ptr())
+                add_g(grad.data_ptr())
+                add_m(st["exp_avg"].data_ptr())
+                add_v(st["exp_avg_sq"].data_ptr())
+                add_lr(lr)
+                add_s(st["state"].data_ptr())
+            lr += 4
         if self.max_norm is not None:
-            self._clipped_step(L, items, tick, gp, stream)
+            self._clipped_step(L, numel, cols, tick, gp, stream)
             return
-        for k in range(0, len(items), 16):
-            chunk = items[k:k + 16]
-            n = len(chunk)
-            numel = (C.c_size_t * n)(*[c[0] for c in chunk])
-            cols = [(C.c_void_p * n)(*[c[j] for c in chunk]) for j in range(1, 7)]
+        for k in range(0, len(numel), 16):                     # one launch per 16 tensors
+            sizes = numel[k:k + 16]
+            n = len(sizes)
+            chunk = [(C.c_void_p * n)(*c[k:k + 16]) for c in cols]
             # step counts / bias corrections advance inside the update launch (the last workgroup of a tensor stores them)
             fn = L.ggs_adam_tick_step_multi if tick else L.ggs_adam_step_multi
-            check(fn(n, numel, cols[0], cols[1], cols[2], cols[3], cols[4], cols[5], b1, b2, self.eps, gp, stream),
+            check(fn(n, (C.c_size_t * n)(*sizes), *chunk, b1, b2, self.eps, gp, stream),
                   "ggs_adam_tick_step_multi" if tick else "ggs_adam_step_multi")
 
-    def _clipped_step(self, L, items, tick: bool, gp, stream) -> None:
-        n = len(items)
-        numel = (C.c_size_t * n)(*[c[0] for c in items])
-        cols = [(C.c_void_p * n)(*[c[j] for c in items]) for j in range(1, 7)]
+    def _clipped_step(self, L, numel, cols, tick: bool, gp, stream) -> None:
+        n = len(numel)
+        addresses = [(C.c_void_p * n)(*c) for c in cols]
         with on_device(self.device):
             # the partial sums of this step: allocated per step, so that two captured steps never share them
             nb = int(L.ggs_grad_norm_workspace_bytes(n))
             ws = torch.empty(nb, dtype=torch.uint8, device=self.device) if nb else None
-            check(L.ggs_adam_clip_step(n, numel, *cols, self.betas[0], self.betas[1], self.eps, _checked_max_norm(self.max_norm),
-                                       int(tick), gp, self.last_grad_norm.data_ptr(), ptr(ws), nb, stream), "ggs_adam_clip_step")
+            check(L.ggs_adam_clip_step(n, (C.c_size_t * n)(*numel), *addresses, self.betas[0], self.betas[1], self.eps,
+                                       _checked_max_norm(self.max_norm), int(tick), gp, self.last_grad_norm.data_ptr(), ptr(ws), nb,
+                                       stream), "ggs_adam_clip_step")

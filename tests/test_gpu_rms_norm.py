@@ -86,7 +86,7 @@ def check(shape, dtype, weight, residual, change=lambda t: t, seed=0):
     return got
 
 
-SHAPES = [(1, 1), (1, 512), (3, 7), (1000, 51), (37, 300), (5, 2050), (2, 10001), (300, 4096), (70000, 8),
+SHAPES = [(1, 1), (1, 512), (3, 7), (1000, 51), (37, 300), (5, 2050), (2, 10001), (3, 16390), (300, 4096), (70000, 8),
           (1, 512, 8, 8), (2, 3, 1, 1), (3, 100, 37, 53), (1, 1, 5, 7), (2, 33, 1, 129), (1, 1030, 3, 5), (2, 1025, 65, 1), (4, 16, 64, 64),
           (2, 5, 9), (1, 8, 2, 3, 5), (2, 257, 20, 9), (1, 32, 3, 700), (5, 64, 4, 4), (1, 600, 31, 33)]
 
@@ -202,7 +202,7 @@ def test_empty_zero_and_not_finite():
 @pytest.mark.parametrize("outer,C,inner", [(3, 51, 1), (7, 515, 1), (2, 9001, 1), (2, 33, 67), (1, 1030, 5), (3, 64, 16), (1, 500, 130)])
 def test_writes_nothing_else(outer, C, inner, dtype):
     """Outputs as windows of larger buffers (at an odd element): what lies in front of and behind them stays as it was."""
-    L, n, pad, code = _lib.lib(), outer * C * inner, 1031, _lib.norm_dtype_code(dtype)
+    L, n, pad, code = _lib.lib(), outer * C * inner, 1031, SN._RMS_TYPES[dtype]
     g = torch.Generator(device="cuda").manual_seed(1)
     x, r, gy, gh = (torch.randn(n, device="cuda", generator=g).to(dtype) for _ in range(4))
     w = torch.ones(C, device="cuda")
