@@ -57,31 +57,33 @@ template <typename A> __device__ __forceinline__ A sum_lanes(A s) {
     return s;
 }
 
-// Any channel count, two passes over the data (the second one from the caches).  PLANES: 64 pixels of one map a workgroup, its
-// four waves take every fourth channel; otherwise one row a workgroup.
+// Any channel count, two passes over the data (the second one from the caches).  PLANES: 64 pixels of one map at a time, the
+// workgroup's four waves take every fourth channel; otherwise one row at a time.
 template <typename T, bool PLANES>
 __global__ __launch_bounds__(256) void k_rms_forward(NormArgs<T> a) {
     typedef typename Acc<T>::type A;
     __shared__ A lds[256];
     const size_t tiles = PLANES ? (a.inner + 63) / 64 : 1;
-    const size_t o = blockIdx.x / tiles, i = PLANES ? (blockIdx.x % tiles) * 64 + (threadIdx.x & 63) : 0;
     const int c0 = PLANES ? threadIdx.x >> 6 : threadIdx.x, step = PLANES ? 4 : 256;
-    const int C = i < a.inner ? a.C : 0;                            // lanes beyond the map only take part in the barriers
-    const size_t base = o * a.C * a.inner + i;
-    A s = 0;
-    for (int c = c0; c < C; c += step) {
-        const A h = value(a, base + c * a.inner);
-        s += h * h;
-    }
-    if (!PLANES) s = sum_lanes(s);
-    s = sum_waves<A>(s, lds);
-    const A q = (A)1 / sqrt(s / (A)a.C + a.eps);
-    if (c0 == 0 && a.q && i < a.inner) a.q[o * a.inner + i] = q;
-    for (int c = c0; c < C; c += step) {
-        const size_t at = base + c * a.inner;
-        const A h = value(a, at);
-        if (a.h) a.h[at] = (T)h;
-        a.y[at] = (T)(weight(a, c) * (h * q));
+    for (size_t tile = blockIdx.x; tile < a.outer * tiles; tile += gridDim.x) {
+        const size_t o = tile / tiles, i = PLANES ? (tile % tiles) * 64 + (threadIdx.x & 63) : 0;
+        const int C = i < a.inner ? a.C : 0;                        // lanes beyond the map only take part in the barriers
+        const size_t base = o * a.C * a.inner + i;
+        A s = 0;
+        for (int c = c0; c < C; c += step) {
+            const A h = value(a, base + c * a.inner);
+            s += h * h;
+        }
+        if (!PLANES) s = sum_lanes(s);
+        s = sum_waves<A>(s, lds);
+        const A q = (A)1 / sqrt(s / (A)a.C + a.eps);
+        if (c0 == 0 && a.q && i < a.inner) a.q[o * a.inner + i] = q;
+        for (int c = c0; c < C; c += step) {
+            const size_t at = base + c * a.inner;
+            const A h = value(a, at);
+            if (a.h) a.h[at] = (T)h;
+            a.y[at] = (T)(weight(a, c) * (h * q));
+        }
     }
 }
 
@@ -90,23 +92,25 @@ __global__ __launch_bounds__(256) void k_rms_backward(NormArgs<T> a) {
     typedef typename Acc<T>::type A;
     __shared__ A lds[256];
     const size_t tiles = PLANES ? (a.inner + 63) / 64 : 1;
-    const size_t o = blockIdx.x / tiles, i = PLANES ? (blockIdx.x % tiles) * 64 + (threadIdx.x & 63) : 0;
     const int c0 = PLANES ? threadIdx.x >> 6 : threadIdx.x, step = PLANES ? 4 : 256;
-    const int C = i < a.inner ? a.C : 0;
-    const size_t base = o * a.C * a.inner + i;
-    const A q = i < a.inner ? a.q[o * a.inner + i] : (A)0;
-    A s = 0;
-    for (int c = c0; c < C; c += step) {
-        const size_t at = base + c * a.inner;
-        s += weight(a, c) * (A)a.gy[at] * (value(a, at) * q);
-    }
-    if (!PLANES) s = sum_lanes(s);
-    s = sum_waves<A>(s, lds) / (A)a.C;
-    for (int c = c0; c < C; c += step) {
-        const size_t at = base + c * a.inner;
-        A d = q * (weight(a, c) * (A)a.gy[at] - value(a, at) * q * s);
-        if (a.gh) d += (A)a.gh[at];
-        a.dx[at] = (T)d;
+    for (size_t tile = blockIdx.x; tile < a.outer * tiles; tile += gridDim.x) {
+        const size_t o = tile / tiles, i = PLANES ? (tile % tiles) * 64 + (threadIdx.x & 63) : 0;
+        const int C = i < a.inner ? a.C : 0;
+        const size_t base = o * a.C * a.inner + i;
+        const A q = i < a.inner ? a.q[o * a.inner + i] : (A)0;
+        A s = 0;
+        for (int c = c0; c < C; c += step) {
+            const size_t at = base + c * a.inner;
+            s += weight(a, c) * (A)a.gy[at] * (value(a, at) * q);
+        }
+        if (!PLANES) s = sum_lanes(s);
+        s = sum_waves<A>(s, lds) / (A)a.C;
+        for (int c = c0; c < C; c += step) {
+            const size_t at = base + c * a.inner;
+            A d = q * (weight(a, c) * (A)a.gy[at] - value(a, at) * q * s);
+            if (a.gh) d += (A)a.gh[at];
+            a.dx[at] = (T)d;
+        }
     }
 }
 
@@ -644,34 +648,71 @@ template <typename T> void one_pass(bool back, const NormArgs<T>& a, const Plan&
 }
 template <> void one_pass<double>(bool, const NormArgs<double>&, const Plan&, hipStream_t) {}
 
+template <typename T> unsigned two_pass_blocks(const NormArgs<T>& a) {
+    const size_t tiles = a.outer * (a.inner == 1 ? 1 : (a.inner + 63) / 64);
+    return (unsigned)(tiles < ((size_t)1 << 22) ? tiles : (size_t)1 << 22);
+}
+
+// Calls launch(a) for as many maps / rows at a time as a launch may have threads for; `threads` is what one of them takes.
+constexpr size_t MAX_THREADS = (size_t)1 << 31;
+template <typename T, typename F> int in_parts(const char* who, const NormArgs<T>& all, size_t threads, F&& launch) {
+    if (threads > MAX_THREADS) return ggs_fail_(GGS_ERR_SIZE, "%s: more than 2^31 threads for one map", who);
+    const size_t per = MAX_THREADS / threads;
+    for (size_t o = 0; o < all.outer; o += per) {
+        NormArgs<T> a = all;
+        a.outer = all.outer - o < per ? all.outer - o : per;
+        const size_t at = o * a.C * a.inner;
+        a.x += at;
+        if (a.r) a.r += at;
+        if (a.gy) a.gy += at;
+        if (a.gh) a.gh += at;
+        if (a.y) a.y += at;
+        if (a.h) a.h += at;
+        if (a.dx) a.dx += at;
+        if (a.q) a.q += o * a.inner;
+        launch(a);
+        const int rc = launched(who);
+        if (rc != GGS_OK) return rc;
+    }
+    return GGS_OK;
+}
+
 template <typename T> int run_forward(NormArgs<T> a, hipStream_t s) {
+    const char* who = "ggs_rms_norm_forward";
     const Plan p = plan<T>(a.outer, a.C, a.inner);
-    const size_t tiles = a.inner == 1 ? 1 : (a.inner + 63) / 64;
-    if (!p.kind && a.outer * tiles > 0x7fffffffu) return ggs_fail_(GGS_ERR_SIZE, "ggs_rms_norm_forward: more than 2^31 workgroups");
-    if (p.kind) one_pass(false, a, p, s);
-    else if (a.inner == 1) hipLaunchKernelGGL((k_rms_forward<T, false>), dim3((unsigned)a.outer), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((k_rms_forward<T, true>), dim3((unsigned)(a.outer * tiles)), dim3(256), 0, s, a);
-    return launched("ggs_rms_norm_forward");
+    if (p.kind) {
+        const size_t threads = p.kind == 2 ? p.lanes : p.tiles / a.outer * p.waves * 64;
+        return in_parts(who, a, threads, [&](const NormArgs<T>& b) {
+            Plan part = p;
+            if (p.kind == 1) part.tiles = p.tiles / a.outer * b.outer;
+            one_pass(false, b, part, s);
+        });
+    }
+    if (a.inner == 1) hipLaunchKernelGGL((k_rms_forward<T, false>), dim3(two_pass_blocks(a)), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_rms_forward<T, true>), dim3(two_pass_blocks(a)), dim3(256), 0, s, a);
+    return launched(who);
 }
 
 template <typename T> int run_backward(NormArgs<T> a, hipStream_t s) {
+    const char* who = "ggs_rms_norm_backward";
     const Plan p = plan<T>(a.outer, a.C, a.inner);
-    const size_t tiles = a.inner == 1 ? 1 : (a.inner + 63) / 64;
-    if (!p.kind && a.outer * tiles > 0x7fffffffu) return ggs_fail_(GGS_ERR_SIZE, "ggs_rms_norm_backward: more than 2^31 workgroups");
-    if (p.kind) one_pass(true, a, p, s);
-    else if (a.inner == 1) hipLaunchKernelGGL((k_rms_backward<T, false>), dim3((unsigned)a.outer), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((k_rms_backward<T, true>), dim3((unsigned)(a.outer * tiles)), dim3(256), 0, s, a);
-    int rc = launched("ggs_rms_norm_backward");
+    if (p.kind) {
+        one_pass(true, a, p, s);
+    } else {
+        if (a.inner == 1) hipLaunchKernelGGL((k_rms_backward<T, false>), dim3(two_pass_blocks(a)), dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((k_rms_backward<T, true>), dim3(two_pass_blocks(a)), dim3(256), 0, s, a);
+    }
+    int rc = launched(who);
     if (rc != GGS_OK || !a.dw) return rc;
     a.n_partial = p.partials;
     if (!p.kind) {
         if (a.inner == 1) hipLaunchKernelGGL((k_rms_dw<T, false>), dim3((a.C + 255) / 256, a.n_partial), dim3(256), 0, s, a);
         else hipLaunchKernelGGL((k_rms_dw<T, true>), dim3(a.C, a.n_partial), dim3(256), 0, s, a);
-        rc = launched("ggs_rms_norm_backward");
+        rc = launched(who);
         if (rc != GGS_OK) return rc;
     }
     hipLaunchKernelGGL((k_rms_dw_sum<T>), dim3((a.C + 7) / 8), dim3(1024), 0, s, a);
-    return launched("ggs_rms_norm_backward");
+    return launched(who);
 }
 
 size_t partials(int dtype, size_t outer, int C, size_t inner) {
@@ -682,6 +723,7 @@ size_t partials(int dtype, size_t outer, int C, size_t inner) {
 int check_sizes(const char* who, int dtype, size_t outer, int channels, size_t inner, double eps) {
     if (dtype < GGS_DTYPE_F32 || dtype > GGS_DTYPE_BF16) return ggs_fail_(GGS_ERR_ARG, "%s: dtype %d is not float / half / double / bfloat16", who, dtype);
     if (channels <= 0) return ggs_fail_(GGS_ERR_ARG, "%s: no channels", who);
+    if (channels > 1 << 22) return ggs_fail_(GGS_ERR_SIZE, "%s: more than 2^22 channels", who);
     if (!(eps > 0.0)) return ggs_fail_(GGS_ERR_ARG, "%s: eps must be positive", who);
     if (inner && outer > ((size_t)1 << 46) / inner / (size_t)channels) return ggs_fail_(GGS_ERR_SIZE, "%s: more than 2^46 elements", who);
     return GGS_OK;

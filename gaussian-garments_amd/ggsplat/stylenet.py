@@ -21,6 +21,7 @@ ggsplat.inner_step.appearance_step: texels are sampled at per-Gaussian UV coordi
 """
 from __future__ import annotations
 
+import functools
 import math
 import os
 from typing import Sequence, Tuple
@@ -205,6 +206,11 @@ def _rms_forward(x, weight, residual, eps, store):
     return y, h, x, residual, weight, q, plan
 
 
+@functools.lru_cache(maxsize=256)
+def _rms_workspace_bytes(code, outer, c, inner):
+    return lib().ggs_rms_norm_workspace_bytes(code, outer, c, inner)
+
+
 class _RmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
@@ -241,7 +247,7 @@ class _RmsNorm(torch.autograd.Function):
         with on_device(dev):
             if need[1]:
                 dw = torch.empty_like(w)
-                nb = L.ggs_rms_norm_workspace_bytes(code, outer, c, inner)
+                nb = _rms_workspace_bytes(code, outer, c, inner)
                 if nb:
                     ws = torch.empty(nb, dtype=torch.uint8, device=dev)
                     dwp, wp = dw.data_ptr(), ws.data_ptr()

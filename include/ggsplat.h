@@ -312,7 +312,7 @@ int ggs_upfirdn2d(int major, int in_h, int in_w, int minor, const float* input, 
  *             computed).  x, residual: as in the forward call, or x = h and residual = NULL (exact in float and double).
  * dtype GGS_DTYPE_*: the type of x, residual, y, h, gy, gh, dx.  weight (NULL: 1) and dw have that type too, or float where
  * weight_f32 != 0.  Sums in float (double for GGS_DTYPE_F64), in an order that does not depend on scheduling.
- * Tensors need no alignment beyond their element's.  workspace (needed with dw): ggs_rms_norm_workspace_bytes(...), any content.
+ * At most 2^22 channels; tensors need no alignment beyond their element's.  workspace (needed with dw): ggs_rms_norm_workspace_bytes(...), any content.
  */
 int ggs_rms_norm_forward(int dtype, size_t outer, int channels, size_t inner, const void* x, const void* residual,
                          const void* weight, int weight_f32, double eps, void* y, void* h, void* q, void* stream);

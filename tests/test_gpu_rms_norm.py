@@ -289,3 +289,36 @@ def test_offsets_beyond_32_bits():
             held("dx", part(dx), ref["dx"], size["dx"], shape[1], 9, torch.float16)
         del x, y, dx, gy, rest
         torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("shape,dtype", [((2 ** 29 + 5, 1), torch.float16), ((2 ** 25 + 3, 1, 3), torch.float16), ((2 ** 23 + 3, 1), torch.float64),
+                                         ((2 ** 23 + 3, 1, 2), torch.float64)], ids=str)
+def test_more_work_than_one_launch_takes(shape, dtype):
+    """2^31 threads and some: rows and maps behind the first launch, and dweight over all of them."""
+    x = torch.empty(shape, device="cuda", dtype=dtype)
+    x.view(-1)[:2 ** 16].normal_(generator=torch.Generator(device="cuda").manual_seed(2))
+    n = x.numel()
+    x.view(-1)[2 ** 16:] = x.view(-1)[:2 ** 16].repeat(n // 2 ** 16 + 1)[:n - 2 ** 16]
+    w = torch.full((1,), 1.5, device="cuda", dtype=torch.float64 if dtype is torch.float64 else torch.float32, requires_grad=True)
+    x.requires_grad_()
+    y = SN.rms_norm(x, w, eps=1.0)
+    dx, dw = torch.autograd.grad(y, (x, w), x.detach())
+    for part in (slice(0, 9), slice(shape[0] // 2, shape[0] // 2 + 9), slice(shape[0] - 9, shape[0])):
+        ref, size = reference(x[part], w, None, x[part], None, eps=1.0)
+        for k, v in (("y", y), ("dx", dx)):
+            held(k, v[part].detach(), ref[k], size[k], 1, 9, dtype)
+    want = 0.0
+    for part in x.detach().view(-1).split(2 ** 26):
+        d = part.double()
+        want += float((d * d / (d * d + 1).sqrt()).sum())
+    # (every term is positive: a thread adds up to 2^29 / 2^16 = 8192 of them one after the other, half a float step each)
+    assert abs(float(dw) - want) <= want * 8200 * 2.0 ** -24, (float(dw), want)
+
+
+def test_gradients_of_two_leaves_do_not_share_memory():
+    x, w, r, gy, gh = tensors((2, 12, 5, 5), torch.float32, "same", True)
+    x.requires_grad_()
+    r.requires_grad_()
+    y, h = SN.rms_norm(x, w, residual=r)
+    torch.autograd.backward((y, h), (gy, gh))
+    assert torch.equal(x.grad, r.grad) and x.grad.data_ptr() != r.grad.data_ptr()

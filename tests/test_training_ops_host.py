@@ -98,6 +98,7 @@ def test_c_entry_points_check_before_any_launch():
     assert "channels" in fwd(0, 1, 0, 1, one, None, None, 0, 1e-8, one, None, None, None)[1]
     assert "eps" in fwd(0, 1, 4, 1, one, None, None, 0, 0.0, one, None, None, None)[1]
     assert "NULL" in fwd(0, 1, 4, 1, None, None, None, 0, 1e-8, one, None, None, None)[1]
+    assert "channels" in fwd(0, 1, (1 << 22) + 1, 1, one, None, None, 0, 1e-8, one, None, None, None)[1]
     assert fwd(0, 1 << 40, 1 << 20, 1 << 40, one, None, None, 0, 1e-8, one, None, None, None)[0] == -3
     assert fwd(0, 0, 4, 1, None, None, None, 0, 1e-8, None, None, None, None)[0] == 0          # nothing to do
     assert L.ggs_rms_norm_workspace_bytes(0, 0, 4, 1) == 0
