@@ -735,6 +735,8 @@ NormArgs<T> norm_args(size_t outer, int channels, size_t inner, const void* x, c
     a.outer = outer; a.inner = inner; a.C = channels;
     a.x = static_cast<const T*>(x); a.r = static_cast<const T*>(residual);
     a.w = weight; a.w32 = weight_f32 != 0; a.eps = (typename Acc<T>::type)eps;
+    const double least = sizeof(T) == 8 ? 2.3e-308 : 1.2e-38;        // in the normal range: a row of zeros gives zeros, not NaN
+    if (a.eps < (typename Acc<T>::type)least) a.eps = (typename Acc<T>::type)least;
     a.inv_c = (typename Acc<T>::type)1 / channels;
     return a;
 }

@@ -22,6 +22,7 @@ import math
 from typing import Dict, Iterable, List, Optional
 
 import torch
+from torch.autograd.graph import increment_version
 
 from ._lib import check, lib, on_device, ptr, stream_ptr
 
@@ -149,6 +150,7 @@ def clip_grad_norm_(grads, max_norm: float, error_if_nonfinite: bool = False) ->
                                   stream_ptr(gl.device)), "ggs_grad_clip")
         for g, c in gl.copies:
             g.copy_(c)
+    increment_version(gl.keep)                     # written in place, as autograd's checks of saved tensors see it
     return norm
 
 
@@ -300,7 +302,7 @@ class GraphAdam:
         gp = ptr(guard)
         b1, b2 = self.betas
         # every tensor that has a gradient: sizes, the six columns of addresses, and the gradients themselves (copies live on)
-        numel, cols, keep, f32 = [], ([], [], [], [], [], []), [], torch.float32
+        numel, cols, keep, params, f32 = [], ([], [], [], [], [], []), [], [], torch.float32
         add_p, add_g, add_m, add_v, add_lr, add_s = (c.append for c in cols)
         states, lr = self.state, self._lr_dev.data_ptr()
         for g in self.param_groups:
@@ -316,6 +318,7 @@ class GraphAdam:
                 st = states[p]
                 numel.append(n)
                 keep.append(grad)
+                params.append(p)
                 add_p(p.data_ptr())
                 add_g(grad.data_ptr())
                 add_m(st["exp_avg"].data_ptr())
@@ -325,6 +328,7 @@ class GraphAdam:
             lr += 4
         if self.max_norm is not None:
             self._clipped_step(L, numel, cols, tick, gp, stream)
+            increment_version(params)
             return
         for k in range(0, len(numel), 16):                     # one launch per 16 tensors
             sizes = numel[k:k + 16]

@@ -352,3 +352,19 @@ def test_captured_clipped_step():
         assert torch.equal(opt.last_grad_norm, ref.last_grad_norm)
         assert all(torch.equal(p, q) for p, q in zip(ps, qs)), k
     assert opt.step_count == 5
+
+
+def test_writes_in_place_are_seen_by_autograd():
+    x = torch.ones(8, device="cuda", requires_grad=True)
+    g = torch.full((8,), 2.0, device="cuda")
+    y = (x * g).sum()                                                            # saves g
+    A.clip_grad_norm_([g], 0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    p = torch.nn.Parameter(torch.ones(8, device="cuda"))
+    opt = A.GraphAdam([p], lr=1e-2, max_norm=1.0)
+    y = (p * p).sum()
+    p.grad = torch.ones_like(p)
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()

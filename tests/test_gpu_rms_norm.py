@@ -184,6 +184,8 @@ def test_empty_zero_and_not_finite():
     z = torch.zeros(2, 6, 3, 3, device="cuda")
     got = passes(z, None, z, z + 1, z)
     assert torch.equal(got["y"], z) and torch.isfinite(got["dx"]).all()
+    for dtype in HALF:                                                           # an eps that a float does not hold
+        assert not SN.rms_norm(z.to(dtype), eps=1e-60).any()
     for shape in ((40, 70), (2, 70, 9, 9), (1, 1100, 3, 3), (9, 9000)):
         x, w, r, gy, gh = tensors(shape, torch.float32, "same", True)
         clean = passes(x, w, r, gy, gh)
