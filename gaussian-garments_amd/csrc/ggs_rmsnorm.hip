@@ -10,6 +10,10 @@
 // Element types float, half, bfloat16 (computed in float) and double (in double).  The backward pass is given h itself in
 // float and double; in 16 bits it is given x and r and adds them again, because the h that was stored is rounded to 8 or 11
 // bits and dw, a sum over all pixels that may be a 32-bit tensor, would carry that rounding.  q is kept in the accumulation type.
+// The backward pass of the backward pass, from the cotangents v of dx and u_c of dw_c, with the means over the channels
+// s = mean(w gy n), b = mean(v n), m = mean(v w gy), t = mean(u gy n):
+//   to gy: w q (v - n b) + u n,   to w: sum over pixels of q gy (v - n b),   to gh: v,
+//   to h:  q^2 (n (3 s b - m) - b w gy - s v) - q n t + q u gy
 // HBM-bound: forward reads x, r and writes y, h; backward reads h (x, r), gy, gh and writes dx: 8 elements a value at most.
 #include "ggs_kernels.h"
 
@@ -22,22 +26,23 @@ template <typename T> struct NormArgs {
     typedef typename Acc<T>::type A;
     size_t outer, inner;
     int C;
-    const T *x, *r, *gy, *gh;
-    const void* w;
-    bool w32;                    // w (and dw) are float whatever T is
+    const T *x, *r, *gy, *gh, *v;
+    const void *w, *u;
+    bool w32;                    // w, u (and dw) are float whatever T is
     A eps, inv_c;                // 1 / C
-    T *y, *h, *dx;
-    A* q;                        // [outer][inner]
+    T *y, *h, *dx, *dgy;
+    A *q, *b;                    // [outer][inner]
     A* partial;                  // [n_partial][C]
     int n_partial;
     void* dw;
 };
 
-template <typename T> __device__ __forceinline__ typename Acc<T>::type weight(const NormArgs<T>& a, int c) {
+template <typename T> __device__ __forceinline__ typename Acc<T>::type per_channel(const NormArgs<T>& a, const void* w, int c, int absent) {
     typedef typename Acc<T>::type A;
-    if (!a.w) return (A)1;
-    return a.w32 ? (A) static_cast<const float*>(a.w)[c] : (A) static_cast<const T*>(a.w)[c];
+    if (!w) return (A)absent;
+    return a.w32 ? (A) static_cast<const float*>(w)[c] : (A) static_cast<const T*>(w)[c];
 }
+template <typename T> __device__ __forceinline__ typename Acc<T>::type weight(const NormArgs<T>& a, int c) { return per_channel(a, a.w, c, 1); }
 template <typename T> __device__ __forceinline__ typename Acc<T>::type value(const NormArgs<T>& a, size_t at) {
     typedef typename Acc<T>::type A;
     return a.r ? (A)a.x[at] + (A)a.r[at] : (A)a.x[at];
@@ -114,9 +119,48 @@ __global__ __launch_bounds__(256) void k_rms_backward(NormArgs<T> a) {
     }
 }
 
-// partial[k][c] = sum of gy n over the k-th share of the pixels.  PLANES: one channel a workgroup; otherwise 256 channels a
-// workgroup, a lane each.
+// The backward pass of the backward pass, in the shape of the two kernels above: four sums, then the gradients to h and gy, and
+// b for k_rms_dw.  No training loop here takes second derivatives every step: kept simple.
 template <typename T, bool PLANES>
+__global__ __launch_bounds__(256) void k_rms_second(NormArgs<T> a) {
+    typedef typename Acc<T>::type A;
+    __shared__ A lds[256];
+    const size_t tiles = PLANES ? (a.inner + 63) / 64 : 1;
+    const int c0 = PLANES ? threadIdx.x >> 6 : threadIdx.x, step = PLANES ? 4 : 256;
+    for (size_t tile = blockIdx.x; tile < a.outer * tiles; tile += gridDim.x) {
+        const size_t o = tile / tiles, i = PLANES ? (tile % tiles) * 64 + (threadIdx.x & 63) : 0;
+        const int C = i < a.inner ? a.C : 0;
+        const size_t base = o * a.C * a.inner + i;
+        const A q = i < a.inner ? a.q[o * a.inner + i] : (A)0;
+        A sum[4] = {};                                              // s, b, m, t
+        for (int c = c0; c < C; c += step) {
+            const size_t at = base + c * a.inner;
+            const A n = value(a, at) * q, g = (A)a.gy[at], w = weight(a, c) * g, v = a.v ? (A)a.v[at] : (A)0;
+            sum[0] += w * n; sum[1] += v * n; sum[2] += v * w; sum[3] += per_channel(a, a.u, c, 0) * g * n;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (!PLANES) sum[k] = sum_lanes(sum[k]);
+            sum[k] = sum_waves<A>(sum[k], lds) / (A)a.C;
+        }
+        if (c0 == 0 && i < a.inner) a.b[o * a.inner + i] = sum[1];
+        for (int c = c0; c < C; c += step) {
+            const size_t at = base + c * a.inner;
+            const A n = value(a, at) * q, g = (A)a.gy[at], w = weight(a, c), v = a.v ? (A)a.v[at] : (A)0, u = per_channel(a, a.u, c, 0);
+            a.dx[at] = (T)(q * (q * (n * ((A)3 * sum[0] * sum[1] - sum[2]) - sum[1] * (w * g) - sum[0] * v) - n * sum[3] + u * g));
+            a.dgy[at] = (T)(w * q * (v - n * sum[1]) + u * n);
+        }
+    }
+}
+
+// partial[k][c] = sum over the k-th share of the pixels of gy n (SECOND: of q gy (v - n b)).  PLANES: one channel a workgroup;
+// otherwise 256 channels a workgroup, a lane each.
+template <typename T, bool SECOND> __device__ __forceinline__ typename Acc<T>::type dw_term(const NormArgs<T>& a, size_t at, size_t p) {
+    typedef typename Acc<T>::type A;
+    const A n = value(a, at) * a.q[p], g = (A)a.gy[at];
+    return SECOND ? a.q[p] * g * ((a.v ? (A)a.v[at] : (A)0) - n * a.b[p]) : g * n;
+}
+template <typename T, bool PLANES, bool SECOND>
 __global__ __launch_bounds__(256) void k_rms_dw(NormArgs<T> a) {
     typedef typename Acc<T>::type A;
     __shared__ A lds[256];
@@ -124,16 +168,14 @@ __global__ __launch_bounds__(256) void k_rms_dw(NormArgs<T> a) {
     A s = 0;
     if (PLANES) {
         const int c = blockIdx.x;
-        for (size_t p = (size_t)blockIdx.y * 256 + threadIdx.x; p < pixels; p += (size_t)gridDim.y * 256) {
-            const size_t at = (p / a.inner * a.C + c) * a.inner + p % a.inner;
-            s += (A)a.gy[at] * (value(a, at) * a.q[p]);
-        }
+        for (size_t p = (size_t)blockIdx.y * 256 + threadIdx.x; p < pixels; p += (size_t)gridDim.y * 256)
+            s += dw_term<T, SECOND>(a, (p / a.inner * a.C + c) * a.inner + p % a.inner, p);
         s = sum_waves<A>(sum_lanes(s), lds);
         if (threadIdx.x == 0) a.partial[(size_t)blockIdx.y * a.C + c] = s;
     } else {
         const int c = blockIdx.x * 256 + threadIdx.x;
         if (c >= a.C) return;
-        for (size_t p = blockIdx.y; p < pixels; p += gridDim.y) s += (A)a.gy[p * a.C + c] * (value(a, p * a.C + c) * a.q[p]);
+        for (size_t p = blockIdx.y; p < pixels; p += gridDim.y) s += dw_term<T, SECOND>(a, p * a.C + c, p);
         a.partial[(size_t)blockIdx.y * a.C + c] = s;
     }
 }
@@ -568,11 +610,13 @@ struct Plan {
     int partials;
 };
 
+int two_pass_partials(size_t pixels) { return (int)(pixels < 64 * 256 ? (pixels + 255) / 256 : 64); }
+
 template <typename T> Plan plan(size_t outer, int C, size_t inner) {
     Plan p = {};
     constexpr int FULL = 16 / sizeof(T);
     const size_t pixels = outer * inner;
-    p.partials = (int)(pixels < 64 * 256 ? (pixels + 255) / 256 : 64);
+    p.partials = two_pass_partials(pixels);
     if (sizeof(T) == 8) return p;
     if (inner == 1) {
         const int vec = C >= FULL ? FULL : 1, vecs = (C + vec - 1) / vec;
@@ -693,6 +737,11 @@ template <typename T> int run_forward(NormArgs<T> a, hipStream_t s) {
     return launched(who);
 }
 
+template <typename T, bool SECOND> void launch_dw(const NormArgs<T>& a, hipStream_t s) {
+    if (a.inner == 1) hipLaunchKernelGGL((k_rms_dw<T, false, SECOND>), dim3((a.C + 255) / 256, a.n_partial), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_rms_dw<T, true, SECOND>), dim3(a.C, a.n_partial), dim3(256), 0, s, a);
+}
+
 template <typename T> int run_backward(NormArgs<T> a, hipStream_t s) {
     const char* who = "ggs_rms_norm_backward";
     const Plan p = plan<T>(a.outer, a.C, a.inner);
@@ -705,12 +754,23 @@ template <typename T> int run_backward(NormArgs<T> a, hipStream_t s) {
     int rc = launched(who);
     if (rc != GGS_OK || !a.dw) return rc;
     a.n_partial = p.partials;
-    if (!p.kind) {
-        if (a.inner == 1) hipLaunchKernelGGL((k_rms_dw<T, false>), dim3((a.C + 255) / 256, a.n_partial), dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((k_rms_dw<T, true>), dim3(a.C, a.n_partial), dim3(256), 0, s, a);
-        rc = launched(who);
-        if (rc != GGS_OK) return rc;
-    }
+    if (!p.kind) launch_dw<T, false>(a, s);
+    rc = launched(who);
+    if (rc != GGS_OK) return rc;
+    hipLaunchKernelGGL((k_rms_dw_sum<T>), dim3((a.C + 7) / 8), dim3(1024), 0, s, a);
+    return launched(who);
+}
+
+template <typename T> int run_second(NormArgs<T> a, hipStream_t s) {
+    const char* who = "ggs_rms_norm_double_backward";
+    if (a.inner == 1) hipLaunchKernelGGL((k_rms_second<T, false>), dim3(two_pass_blocks(a)), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_rms_second<T, true>), dim3(two_pass_blocks(a)), dim3(256), 0, s, a);
+    int rc = launched(who);
+    if (rc != GGS_OK || !a.dw) return rc;
+    a.n_partial = two_pass_partials(a.outer * a.inner);
+    launch_dw<T, true>(a, s);
+    rc = launched(who);
+    if (rc != GGS_OK) return rc;
     hipLaunchKernelGGL((k_rms_dw_sum<T>), dim3((a.C + 7) / 8), dim3(1024), 0, s, a);
     return launched(who);
 }
@@ -759,6 +819,23 @@ int backward(size_t outer, int channels, size_t inner, const void* x, const void
     return run_backward(a, s);
 }
 
+// Workspace of the double backward pass: b of every pixel, then the partials.
+size_t second_bytes(int dtype, size_t outer, int channels, size_t inner) {
+    const size_t pixels = outer * inner;
+    return (pixels + (size_t)two_pass_partials(pixels) * channels) * (dtype == GGS_DTYPE_F64 ? 8 : 4);
+}
+
+template <typename T>
+int second(size_t outer, int channels, size_t inner, const void* x, const void* residual, const void* weight, int weight_f32, const void* q,
+           const void* gy, const void* v, const void* u, void* dh, void* dgy, void* dw, void* workspace, hipStream_t s) {
+    NormArgs<T> a = norm_args<T>(outer, channels, inner, x, residual, weight, weight_f32, 0.0);
+    a.q = static_cast<typename Acc<T>::type*>(const_cast<void*>(q));
+    a.gy = static_cast<const T*>(gy); a.v = static_cast<const T*>(v); a.u = u;
+    a.dx = static_cast<T*>(dh); a.dgy = static_cast<T*>(dgy); a.dw = dw;
+    a.b = static_cast<typename Acc<T>::type*>(workspace); a.partial = a.b + outer * inner;
+    return run_second(a, s);
+}
+
 }  // namespace
 
 extern "C" {
@@ -800,6 +877,29 @@ int ggs_rms_norm_backward(int dtype, size_t outer, int channels, size_t inner, c
         case GGS_DTYPE_F16: return backward<_Float16>(outer, channels, inner, x, residual, weight, weight_f32, q, gy, gh, dx, dw, workspace, s);
         case GGS_DTYPE_BF16: return backward<__bf16>(outer, channels, inner, x, residual, weight, weight_f32, q, gy, gh, dx, dw, workspace, s);
         default: return backward<double>(outer, channels, inner, x, residual, weight, weight_f32, q, gy, gh, dx, dw, workspace, s);
+    }
+}
+
+size_t ggs_rms_norm_double_workspace_bytes(int dtype, size_t outer, int channels, size_t inner) {
+    return channels <= 0 || outer == 0 || inner == 0 ? 0 : second_bytes(dtype, outer, channels, inner);
+}
+
+int ggs_rms_norm_double_backward(int dtype, size_t outer, int channels, size_t inner, const void* x, const void* residual,
+                                 const void* weight, int weight_f32, const void* q, const void* gy, const void* v, const void* u,
+                                 void* dh, void* dgy, void* dw, void* workspace, size_t workspace_bytes, void* stream) {
+    ggs_clear_error_();
+    int rc = check_sizes("ggs_rms_norm_double_backward", dtype, outer, channels, inner, 1.0);
+    if (rc != GGS_OK) return rc;
+    if (outer == 0 || inner == 0) return GGS_OK;
+    if (!x || !q || !gy || !dh || !dgy) return ggs_fail_(GGS_ERR_ARG, "ggs_rms_norm_double_backward: NULL pointer argument");
+    if (!workspace || workspace_bytes < second_bytes(dtype, outer, channels, inner))
+        return ggs_fail_(GGS_ERR_SIZE, "ggs_rms_norm_double_backward: the workspace is too small (ggs_rms_norm_double_workspace_bytes)");
+    hipStream_t s = (hipStream_t)stream;
+    switch (dtype) {
+        case GGS_DTYPE_F32: return second<float>(outer, channels, inner, x, residual, weight, weight_f32, q, gy, v, u, dh, dgy, dw, workspace, s);
+        case GGS_DTYPE_F16: return second<_Float16>(outer, channels, inner, x, residual, weight, weight_f32, q, gy, v, u, dh, dgy, dw, workspace, s);
+        case GGS_DTYPE_BF16: return second<__bf16>(outer, channels, inner, x, residual, weight, weight_f32, q, gy, v, u, dh, dgy, dw, workspace, s);
+        default: return second<double>(outer, channels, inner, x, residual, weight, weight_f32, q, gy, v, u, dh, dgy, dw, workspace, s);
     }
 }
 

@@ -78,6 +78,8 @@ _SIGS = {
     "ggs_rms_norm_forward": (C.c_int, [C.c_int, C.c_size_t, C.c_int, C.c_size_t] + [_PTR] * 3 + [C.c_int, C.c_double] + [_PTR] * 4),
     "ggs_rms_norm_workspace_bytes": (C.c_size_t, [C.c_int, C.c_size_t, C.c_int, C.c_size_t]),
     "ggs_rms_norm_backward": (C.c_int, [C.c_int, C.c_size_t, C.c_int, C.c_size_t] + [_PTR] * 3 + [C.c_int] + [_PTR] * 6 + [C.c_size_t, _PTR]),
+    "ggs_rms_norm_double_workspace_bytes": (C.c_size_t, [C.c_int, C.c_size_t, C.c_int, C.c_size_t]),
+    "ggs_rms_norm_double_backward": (C.c_int, [C.c_int, C.c_size_t, C.c_int, C.c_size_t] + [_PTR] * 3 + [C.c_int] + [_PTR] * 8 + [C.c_size_t, _PTR]),
     "ggs_adam_state_bytes": (C.c_size_t, []),
     "ggs_adam_tick": (C.c_int, [_PTR, C.c_double, C.c_double, _PTR, _PTR]),
     "ggs_adam_step": (C.c_int, [C.c_size_t, _PTR, _PTR, _PTR, _PTR, _PTR, C.c_double, C.c_double, C.c_double, _PTR, _PTR, _PTR]),

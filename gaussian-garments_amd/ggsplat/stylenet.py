@@ -155,6 +155,7 @@ def resample2d(x, k, up: int = 1, down: int = 1, pad: Tuple[int, int] = (0, 0), 
 # op 3: root-mean-square norm over the channels ("pixel norm") with the residual's addition
 #   h = x + residual,  q = (mean_c h^2 + eps)^-1/2,  y = weight q h;   with n = q h:
 #   dL/dh = q (weight gy - n mean_c(weight gy n)) + gh = dL/dx = dL/dresidual,   dL/dweight = sum over pixels of gy n
+#   (second derivatives: csrc/ggs_rmsnorm.hip)
 # ------------------------------------------------------------------------------------------------------------------
 _RMS_TYPES = {torch.float32: 0, torch.float16: 1, torch.float64: 2, torch.bfloat16: 3}      # GGS_DTYPE_*
 
@@ -228,34 +229,77 @@ class _RmsNorm(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, gy, gh=None):
-        if torch.is_grad_enabled():                                   # create_graph=True
-            raise RuntimeError("rms_norm: its gradients are not differentiable again (create_graph=True)")
         need = ctx.needs_input_grad
         if gy is None:                                                # only h was used further on
             return gh, None, gh if need[2] else None, None
         x, residual, w, q = ctx.saved_tensors
-        code, outer, c, inner, w32, rows = ctx.plan
-        gy = _rms_order(gy, rows)
-        gp = rp = dw = dwp = wp = None
-        if gh is not None:
-            gh = _rms_order(gh, rows)
-            gp = gh.data_ptr()
-        if residual is not None:
-            rp = residual.data_ptr()
-        dx = torch.empty_like(x)
-        dev, nb, L = x.device, 0, lib()
-        with on_device(dev):
-            if need[1]:
-                dw = torch.empty_like(w)
-                nb = _rms_workspace_bytes(code, outer, c, inner)
-                if nb:
-                    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
-                    dwp, wp = dw.data_ptr(), ws.data_ptr()
-                else:
-                    dw.zero_()                                        # no pixels
-            check(L.ggs_rms_norm_backward(code, outer, c, inner, x.data_ptr(), rp, ptr(w), w32, q.data_ptr(), gy.data_ptr(), gp,
-                                          dx.data_ptr(), dwp, wp, nb, stream_ptr(dev)), "ggs_rms_norm_backward")
+        if torch.is_grad_enabled():                                   # create_graph=True
+            dx, dw = _RmsNormGrad.apply(x, residual, w, q, gy, gh, ctx.plan, need[1])
+        else:
+            dx, dw = _rms_backward(x, residual, w, q, gy, gh, ctx.plan, need[1])[:2]
         return dx, dw, dx if need[2] else None, None
+
+
+def _rms_backward(x, residual, w, q, gy, gh, plan, need_dw):
+    """(dx, dw or None, gy in the kernels' order)"""
+    code, outer, c, inner, w32, rows = plan
+    gy = _rms_order(gy, rows)
+    gp = rp = dw = dwp = wp = None
+    if gh is not None:
+        gh = _rms_order(gh, rows)
+        gp = gh.data_ptr()
+    if residual is not None:
+        rp = residual.data_ptr()
+    dx = torch.empty_like(x)
+    dev, nb, L = x.device, 0, lib()
+    with on_device(dev):
+        if need_dw:
+            dw = torch.empty_like(w)
+            nb = _rms_workspace_bytes(code, outer, c, inner)
+            if nb:
+                ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+                dwp, wp = dw.data_ptr(), ws.data_ptr()
+            else:
+                dw.zero_()                                            # no pixels
+        check(L.ggs_rms_norm_backward(code, outer, c, inner, x.data_ptr(), rp, ptr(w), w32, q.data_ptr(), gy.data_ptr(), gp,
+                                      dx.data_ptr(), dwp, wp, nb, stream_ptr(dev)), "ggs_rms_norm_backward")
+    return dx, dw, gy
+
+
+class _RmsNormGrad(torch.autograd.Function):
+    """The backward pass as a Function of its own, for second derivatives.  (q depends on x; the gradient to x accounts for it.)"""
+
+    @staticmethod
+    def forward(ctx, x, residual, w, q, gy, gh, plan, need_dw):
+        dx, dw, gy = _rms_backward(x, residual, w, q, gy, gh, plan, need_dw)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x, residual, w, q, gy)
+        ctx.plan = plan
+        return dx, dw
+
+    @staticmethod
+    def backward(ctx, v, u):
+        if torch.is_grad_enabled():
+            raise RuntimeError("rms_norm: its second derivatives are not differentiable again (create_graph=True)")
+        if v is None and u is None:
+            return (None,) * 8
+        x, residual, w, q, gy = ctx.saved_tensors
+        code, outer, c, inner, w32, rows = ctx.plan
+        need = ctx.needs_input_grad
+        v = None if v is None else _rms_order(v, rows)
+        u = None if u is None else u.contiguous()
+        dh, dgy, L, dev = torch.empty_like(x), torch.empty_like(x), lib(), x.device
+        dw = torch.empty_like(w) if w is not None and need[2] else None
+        with on_device(dev):
+            nb = L.ggs_rms_norm_double_workspace_bytes(code, outer, c, inner)
+            ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+            if dw is not None and nb == 0:
+                dw.zero_()                                            # no pixels
+            check(L.ggs_rms_norm_double_backward(code, outer, c, inner, x.data_ptr(), None if residual is None else residual.data_ptr(),
+                                                 ptr(w), w32, q.data_ptr(), gy.data_ptr(), None if v is None else v.data_ptr(), ptr(u),
+                                                 dh.data_ptr(), dgy.data_ptr(), ptr(dw), ws.data_ptr(), nb, stream_ptr(dev)),
+                  "ggs_rms_norm_double_backward")
+        return dh, dh if need[1] else None, dw, None, dgy if need[4] else None, v if need[5] else None, None, None
 
 
 def rms_norm(x, weight=None, residual=None, eps: float = 1e-8, impl: str = "hip"):
@@ -263,7 +307,7 @@ def rms_norm(x, weight=None, residual=None, eps: float = 1e-8, impl: str = "hip"
     feature map by itself; [rows, C]: every row).  Returns y, or (y, h) with a residual -- h is the sum to carry on.
     x, residual: float32 / float16 / bfloat16 / float64, the same shape; weight [C]: x's type or float32; contiguous and
     channels-last maps are taken as they are.  The norm is that of the unrounded sum; sums are in float (double for float64).
-    Differentiable once (its gradients are not differentiable again)."""
+    Differentiable twice (second derivatives are not differentiable again)."""
     shape, dtype = x.shape, x.dtype
     if len(shape) < 2 or shape[1] == 0:
         raise ValueError(f"rms_norm: x must be [B, C, ...] with C > 0, got {tuple(shape)}")

@@ -310,9 +310,13 @@ int ggs_upfirdn2d(int major, int in_h, int in_w, int minor, const float* input, 
  *             backward pass needs.  The norm is that of the sum before `h` is rounded to the element type.
  *   backward: dx = dL/dx = dL/dresidual from gy = dL/dy and gh = dL/dh (NULL: none); dw [channels] = dL/dweight (NULL: not
  *             computed).  x, residual: as in the forward call, or x = h and residual = NULL (exact in float and double).
- * dtype GGS_DTYPE_*: the type of x, residual, y, h, gy, gh, dx.  weight (NULL: 1) and dw have that type too, or float where
- * weight_f32 != 0.  Sums in float (double for GGS_DTYPE_F64), in an order that does not depend on scheduling.
- * At most 2^22 channels; tensors need no alignment beyond their element's.  workspace (needed with dw): ggs_rms_norm_workspace_bytes(...), any content.
+ *   double_backward: the backward pass of the backward pass: from v = cotangent of dx (NULL: zeros) and u [channels] = cotangent
+ *             of dw (NULL: zeros) the gradients dh (to x and residual alike), dgy (to gy) and dw (to weight; NULL: not
+ *             computed); that to gh is v.
+ * dtype GGS_DTYPE_*: the type of x, residual, y, h, gy, gh, dx, v, dh, dgy.  weight (NULL: 1), u and dw have that type too, or
+ * float where weight_f32 != 0.  Sums in float (double for GGS_DTYPE_F64), in an order that does not depend on scheduling.
+ * At most 2^22 channels; tensors need no alignment beyond their element's.  workspace (backward: needed with
+ * dw): ggs_rms_norm_workspace_bytes / _double_workspace_bytes(...) bytes, 8-byte aligned, any content.
  */
 int ggs_rms_norm_forward(int dtype, size_t outer, int channels, size_t inner, const void* x, const void* residual,
                          const void* weight, int weight_f32, double eps, void* y, void* h, void* q, void* stream);
@@ -320,6 +324,10 @@ size_t ggs_rms_norm_workspace_bytes(int dtype, size_t outer, int channels, size_
 int ggs_rms_norm_backward(int dtype, size_t outer, int channels, size_t inner, const void* x, const void* residual,
                           const void* weight, int weight_f32, const void* q, const void* gy, const void* gh, void* dx,
                           void* dw, void* workspace, size_t workspace_bytes, void* stream);
+size_t ggs_rms_norm_double_workspace_bytes(int dtype, size_t outer, int channels, size_t inner);
+int ggs_rms_norm_double_backward(int dtype, size_t outer, int channels, size_t inner, const void* x, const void* residual,
+                                 const void* weight, int weight_f32, const void* q, const void* gy, const void* v, const void* u,
+                                 void* dh, void* dgy, void* dw, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Optimiser update of the inner loops as graph-capturable kernels -- what the reference does with

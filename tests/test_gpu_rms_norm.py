@@ -148,6 +148,50 @@ def test_gradients_against_differences():
         assert torch.autograd.gradcheck(lambda a: SN.rms_norm(a, eps=1e-3), (x,))
 
 
+def test_second_derivatives_against_differences():
+    g = torch.Generator().manual_seed(8)
+    for shape in ((3, 5), (2, 6, 3, 2), (2, 70, 2, 1), (300, 2, 3)):
+        x, r, gy, gh = (torch.randn(*shape, generator=g, dtype=torch.float64).cuda().requires_grad_() for _ in range(4))
+        w = torch.randn(shape[1], generator=g, dtype=torch.float64).cuda().requires_grad_()
+        fast = dict(fast_mode=True) if x.numel() > 100 else {}
+        assert torch.autograd.gradgradcheck(lambda a, b, c: SN.rms_norm(a, b, residual=c, eps=1e-2), (x, w, r), (gy, gh), **fast)
+        assert torch.autograd.gradgradcheck(lambda a, b: SN.rms_norm(a, b, eps=1e-2), (x, w), (gy,), **fast)
+        assert torch.autograd.gradgradcheck(lambda a: SN.rms_norm(a, eps=1e-2), (x,), (gy,), **fast)
+        last = x.detach().movedim(1, -1).contiguous().movedim(-1, 1).requires_grad_()
+        assert torch.autograd.gradgradcheck(lambda a, b: SN.rms_norm(a, b, eps=1e-2), (last, w), (gy,), **fast)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("shape", [(40, 51), (2, 65, 9, 7), (3, 1030, 2, 2)], ids=str)
+def test_second_derivatives(shape, dtype):
+    """A gradient penalty's gradients against the same through the plain form in double.  Every value passes two normalisations:
+    off by at most 2 (C + 16) a of the largest magnitudes that enter and u once (16 bits: dx and dw, whose squares the penalty sums,
+    are rounded on the way, u each); compared in norm, where independent roundings do not add up."""
+    x, w, r, gy, gh = tensors(shape, dtype, "float32", True, seed=9)
+    got = []
+    for impl, cast in (("hip", lambda t: t), ("native", lambda t: t.double())):
+        leaves = [cast(t).detach().requires_grad_() for t in (x, w, r, gy, gh)]
+        y, h = SN.rms_norm(leaves[0], leaves[1], residual=leaves[2], impl=impl)
+        gx, gw = torch.autograd.grad((y, h), leaves[:2], (leaves[3], leaves[4]), create_graph=True)
+        if impl == "native":                                                    # the cotangents the other side works with
+            gx, gw = gx + (first[0].double() - gx).detach(), gw + (first[1].double() - gw).detach()
+        else:
+            first = (gx.detach(), gw.detach())
+        got.append(torch.autograd.grad((gx.double().square().sum() + gw.double().square().sum()) / 2, leaves))
+    for name, a, b in zip(("x", "w", "r", "gy", "gh"), *got):
+        assert a.shape == b.shape
+        off = float((a.double() - b).norm() / b.norm())
+        assert off <= 2 * HALF[dtype] + 2 * (shape[1] + 16) * HALF[torch.float32], (name, off)
+
+
+def test_third_derivatives_are_refused():
+    x = torch.randn(4, 6, device="cuda", requires_grad=True)
+    (g,) = torch.autograd.grad(SN.rms_norm(x).sin().sum(), x, create_graph=True)
+    torch.autograd.grad(g.square().sum(), x, retain_graph=True)
+    with pytest.raises(RuntimeError, match="not differentiable again"):
+        torch.autograd.grad(g.square().sum(), x, create_graph=True)
+
+
 def test_which_gradients_are_asked_for():
     x, w, r, gy, gh = tensors((2, 12, 5, 5), torch.float32, "same", True)
     full = passes(x, w, r, gy, gh)
@@ -169,8 +213,6 @@ def test_which_gradients_are_asked_for():
     (ga,) = torch.autograd.grad((y, h), a, (gy, gh))
     ref, size = reference(x, w, x, gy, gh)
     held("dx", ga, 2 * ref["dx"], 2 * size["dx"], 12, 50, torch.float32)
-    with pytest.raises(RuntimeError, match="not differentiable again"):
-        torch.autograd.grad(SN.rms_norm(a, w).sum(), a, create_graph=True)
 
 
 def test_empty_zero_and_not_finite():

@@ -107,6 +107,11 @@ def test_c_entry_points_check_before_any_launch():
     bwd = lambda *a: _rc(L.ggs_rms_norm_backward, *a)              # noqa: E731
     assert "workspace" in bwd(0, 1000, 64, 7, one, None, one, 0, one, one, None, one, one, one, nb - 1, None)[1]
     assert "NULL" in bwd(0, 1000, 64, 7, one, None, one, 0, None, one, None, one, None, None, 0, None)[1]
+    two = lambda *a: _rc(L.ggs_rms_norm_double_backward, *a)       # noqa: E731
+    nb = L.ggs_rms_norm_double_workspace_bytes(0, 1000, 64, 7)
+    assert nb >= 4 * 7000 and L.ggs_rms_norm_double_workspace_bytes(2, 1000, 64, 7) == 2 * nb
+    assert "workspace" in two(0, 1000, 64, 7, one, None, one, 0, one, one, one, None, one, one, one, one, nb - 1, None)[1]
+    assert "NULL" in two(0, 1000, 64, 7, one, None, one, 0, one, None, one, None, one, one, one, one, nb, None)[1]
 
 
 def test_training_setup_clips_only_with_the_gpu_optimiser():
