@@ -48,13 +48,16 @@ template <typename T> __device__ __forceinline__ typename Acc<T>::type value(con
     return a.r ? (A)a.x[at] + (A)a.r[at] : (A)a.x[at];
 }
 
-// Sum over the 4 waves of a workgroup, lane by lane.
-template <typename A> __device__ __forceinline__ A sum_waves(A s, A* lds) {
+// Sum over the W waves of a workgroup, lane by lane.
+template <int W, typename A> __device__ __forceinline__ A sum_waves(A s, A* lds) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     __syncthreads();
     lds[wave * 64 + lane] = s;
     __syncthreads();
-    return (lds[lane] + lds[64 + lane]) + (lds[128 + lane] + lds[192 + lane]);
+    s = 0;
+#pragma unroll
+    for (int k = 0; k < W; ++k) s += lds[k * 64 + lane];
+    return s;
 }
 template <typename A> __device__ __forceinline__ A sum_lanes(A s) {
 #pragma unroll
@@ -63,13 +66,13 @@ template <typename A> __device__ __forceinline__ A sum_lanes(A s) {
 }
 
 // Any channel count, two passes over the data (the second one from the caches).  PLANES: 64 pixels of one map at a time, the
-// workgroup's four waves take every fourth channel; otherwise one row at a time.
+// workgroup's sixteen waves take every sixteenth channel; otherwise one row at a time.
 template <typename T, bool PLANES>
-__global__ __launch_bounds__(256) void k_rms_forward(NormArgs<T> a) {
+__global__ __launch_bounds__(1024) void k_rms_forward(NormArgs<T> a) {
     typedef typename Acc<T>::type A;
-    __shared__ A lds[256];
+    __shared__ A lds[1024];
     const size_t tiles = PLANES ? (a.inner + 63) / 64 : 1;
-    const int c0 = PLANES ? threadIdx.x >> 6 : threadIdx.x, step = PLANES ? 4 : 256;
+    const int c0 = PLANES ? threadIdx.x >> 6 : threadIdx.x, step = PLANES ? 16 : 1024;
     for (size_t tile = blockIdx.x; tile < a.outer * tiles; tile += gridDim.x) {
         const size_t o = tile / tiles, i = PLANES ? (tile % tiles) * 64 + (threadIdx.x & 63) : 0;
         const int C = i < a.inner ? a.C : 0;                        // lanes beyond the map only take part in the barriers
@@ -80,7 +83,7 @@ __global__ __launch_bounds__(256) void k_rms_forward(NormArgs<T> a) {
             s += h * h;
         }
         if (!PLANES) s = sum_lanes(s);
-        s = sum_waves<A>(s, lds);
+        s = sum_waves<16>(s, lds);
         const A q = (A)1 / sqrt(s / (A)a.C + a.eps);
         if (c0 == 0 && a.q && i < a.inner) a.q[o * a.inner + i] = q;
         for (int c = c0; c < C; c += step) {
@@ -93,11 +96,11 @@ __global__ __launch_bounds__(256) void k_rms_forward(NormArgs<T> a) {
 }
 
 template <typename T, bool PLANES>
-__global__ __launch_bounds__(256) void k_rms_backward(NormArgs<T> a) {
+__global__ __launch_bounds__(1024) void k_rms_backward(NormArgs<T> a) {
     typedef typename Acc<T>::type A;
-    __shared__ A lds[256];
+    __shared__ A lds[1024];
     const size_t tiles = PLANES ? (a.inner + 63) / 64 : 1;
-    const int c0 = PLANES ? threadIdx.x >> 6 : threadIdx.x, step = PLANES ? 4 : 256;
+    const int c0 = PLANES ? threadIdx.x >> 6 : threadIdx.x, step = PLANES ? 16 : 1024;
     for (size_t tile = blockIdx.x; tile < a.outer * tiles; tile += gridDim.x) {
         const size_t o = tile / tiles, i = PLANES ? (tile % tiles) * 64 + (threadIdx.x & 63) : 0;
         const int C = i < a.inner ? a.C : 0;
@@ -109,7 +112,7 @@ __global__ __launch_bounds__(256) void k_rms_backward(NormArgs<T> a) {
             s += weight(a, c) * (A)a.gy[at] * (value(a, at) * q);
         }
         if (!PLANES) s = sum_lanes(s);
-        s = sum_waves<A>(s, lds) / (A)a.C;
+        s = sum_waves<16>(s, lds) / (A)a.C;
         for (int c = c0; c < C; c += step) {
             const size_t at = base + c * a.inner;
             A d = q * (weight(a, c) * (A)a.gy[at] - value(a, at) * q * s);
@@ -122,11 +125,11 @@ __global__ __launch_bounds__(256) void k_rms_backward(NormArgs<T> a) {
 // The backward pass of the backward pass, in the shape of the two kernels above: four sums, then the gradients to h and gy, and
 // b for k_rms_dw.  No training loop here takes second derivatives every step: kept simple.
 template <typename T, bool PLANES>
-__global__ __launch_bounds__(256) void k_rms_second(NormArgs<T> a) {
+__global__ __launch_bounds__(1024) void k_rms_second(NormArgs<T> a) {
     typedef typename Acc<T>::type A;
-    __shared__ A lds[256];
+    __shared__ A lds[1024];
     const size_t tiles = PLANES ? (a.inner + 63) / 64 : 1;
-    const int c0 = PLANES ? threadIdx.x >> 6 : threadIdx.x, step = PLANES ? 4 : 256;
+    const int c0 = PLANES ? threadIdx.x >> 6 : threadIdx.x, step = PLANES ? 16 : 1024;
     for (size_t tile = blockIdx.x; tile < a.outer * tiles; tile += gridDim.x) {
         const size_t o = tile / tiles, i = PLANES ? (tile % tiles) * 64 + (threadIdx.x & 63) : 0;
         const int C = i < a.inner ? a.C : 0;
@@ -141,7 +144,7 @@ __global__ __launch_bounds__(256) void k_rms_second(NormArgs<T> a) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             if (!PLANES) sum[k] = sum_lanes(sum[k]);
-            sum[k] = sum_waves<A>(sum[k], lds) / (A)a.C;
+            sum[k] = sum_waves<16>(sum[k], lds) / (A)a.C;
         }
         if (c0 == 0 && i < a.inner) a.b[o * a.inner + i] = sum[1];
         for (int c = c0; c < C; c += step) {
@@ -170,7 +173,7 @@ __global__ __launch_bounds__(256) void k_rms_dw(NormArgs<T> a) {
         const int c = blockIdx.x;
         for (size_t p = (size_t)blockIdx.y * 256 + threadIdx.x; p < pixels; p += (size_t)gridDim.y * 256)
             s += dw_term<T, SECOND>(a, (p / a.inner * a.C + c) * a.inner + p % a.inner, p);
-        s = sum_waves<A>(sum_lanes(s), lds);
+        s = sum_waves<4>(sum_lanes(s), lds);
         if (threadIdx.x == 0) a.partial[(size_t)blockIdx.y * a.C + c] = s;
     } else {
         const int c = blockIdx.x * 256 + threadIdx.x;
@@ -610,13 +613,17 @@ struct Plan {
     int partials;
 };
 
-int two_pass_partials(size_t pixels) { return (int)(pixels < 64 * 256 ? (pixels + 255) / 256 : 64); }
+// Shares of the pixels in k_rms_dw: 256 pixels each and at most 64 for maps, 16 each and at most 256 for rows.
+int two_pass_partials(size_t outer, size_t inner) {
+    const size_t each = inner == 1 ? 16 : 256, most = inner == 1 ? 256 : 64, n = (outer * inner + each - 1) / each;
+    return (int)(n < most ? n : most);
+}
 
 template <typename T> Plan plan(size_t outer, int C, size_t inner) {
     Plan p = {};
     constexpr int FULL = 16 / sizeof(T);
     const size_t pixels = outer * inner;
-    p.partials = two_pass_partials(pixels);
+    p.partials = two_pass_partials(outer, inner);
     if (sizeof(T) == 8) return p;
     if (inner == 1) {
         const int vec = C >= FULL ? FULL : 1, vecs = (C + vec - 1) / vec;
@@ -694,7 +701,7 @@ template <> void one_pass<double>(bool, const NormArgs<double>&, const Plan&, hi
 
 template <typename T> unsigned two_pass_blocks(const NormArgs<T>& a) {
     const size_t tiles = a.outer * (a.inner == 1 ? 1 : (a.inner + 63) / 64);
-    return (unsigned)(tiles < ((size_t)1 << 22) ? tiles : (size_t)1 << 22);
+    return (unsigned)(tiles < ((size_t)1 << 20) ? tiles : (size_t)1 << 20);
 }
 
 // Calls launch(a) for as many maps / rows at a time as a launch may have threads for; `threads` is what one of them takes.
@@ -732,8 +739,8 @@ template <typename T> int run_forward(NormArgs<T> a, hipStream_t s) {
             one_pass(false, b, part, s);
         });
     }
-    if (a.inner == 1) hipLaunchKernelGGL((k_rms_forward<T, false>), dim3(two_pass_blocks(a)), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((k_rms_forward<T, true>), dim3(two_pass_blocks(a)), dim3(256), 0, s, a);
+    if (a.inner == 1) hipLaunchKernelGGL((k_rms_forward<T, false>), dim3(two_pass_blocks(a)), dim3(1024), 0, s, a);
+    else hipLaunchKernelGGL((k_rms_forward<T, true>), dim3(two_pass_blocks(a)), dim3(1024), 0, s, a);
     return launched(who);
 }
 
@@ -748,8 +755,8 @@ template <typename T> int run_backward(NormArgs<T> a, hipStream_t s) {
     if (p.kind) {
         one_pass(true, a, p, s);
     } else {
-        if (a.inner == 1) hipLaunchKernelGGL((k_rms_backward<T, false>), dim3(two_pass_blocks(a)), dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((k_rms_backward<T, true>), dim3(two_pass_blocks(a)), dim3(256), 0, s, a);
+        if (a.inner == 1) hipLaunchKernelGGL((k_rms_backward<T, false>), dim3(two_pass_blocks(a)), dim3(1024), 0, s, a);
+        else hipLaunchKernelGGL((k_rms_backward<T, true>), dim3(two_pass_blocks(a)), dim3(1024), 0, s, a);
     }
     int rc = launched(who);
     if (rc != GGS_OK || !a.dw) return rc;
@@ -763,11 +770,11 @@ template <typename T> int run_backward(NormArgs<T> a, hipStream_t s) {
 
 template <typename T> int run_second(NormArgs<T> a, hipStream_t s) {
     const char* who = "ggs_rms_norm_double_backward";
-    if (a.inner == 1) hipLaunchKernelGGL((k_rms_second<T, false>), dim3(two_pass_blocks(a)), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((k_rms_second<T, true>), dim3(two_pass_blocks(a)), dim3(256), 0, s, a);
+    if (a.inner == 1) hipLaunchKernelGGL((k_rms_second<T, false>), dim3(two_pass_blocks(a)), dim3(1024), 0, s, a);
+    else hipLaunchKernelGGL((k_rms_second<T, true>), dim3(two_pass_blocks(a)), dim3(1024), 0, s, a);
     int rc = launched(who);
     if (rc != GGS_OK || !a.dw) return rc;
-    a.n_partial = two_pass_partials(a.outer * a.inner);
+    a.n_partial = two_pass_partials(a.outer, a.inner);
     launch_dw<T, true>(a, s);
     rc = launched(who);
     if (rc != GGS_OK) return rc;
@@ -822,7 +829,7 @@ int backward(size_t outer, int channels, size_t inner, const void* x, const void
 // Workspace of the double backward pass: b of every pixel, then the partials.
 size_t second_bytes(int dtype, size_t outer, int channels, size_t inner) {
     const size_t pixels = outer * inner;
-    return (pixels + (size_t)two_pass_partials(pixels) * channels) * (dtype == GGS_DTYPE_F64 ? 8 : 4);
+    return (pixels + (size_t)two_pass_partials(outer, inner) * channels) * (dtype == GGS_DTYPE_F64 ? 8 : 4);
 }
 
 template <typename T>
