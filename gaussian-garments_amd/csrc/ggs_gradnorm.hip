@@ -11,6 +11,12 @@
 // (5 elements a clock per CU) the conversions and fused multiply-adds fill less than half of the vector pipes.
 // HBM-bound: the norm reads every gradient once, the scaling reads and writes it once (nothing when c = 1), the update moves
 // ggs_adam.hip's 28 bytes an element.
+// Measured (replayed from a graph, inputs of three passes in turn; a copy of 2 GiB runs at 4.9 TB/s here):
+//   norm of 43.8M float gradients (78 tensors)           36.7 us with the skipped scaling: 4.8 TB/s
+//   norm and scaling of 43.8M bf16 gradients             38.9 us: 263 MB moved, the second read from the caches
+//   norm and scaling of 6.05M float gradients (7)        11.1 us: two launches and 73 MB
+//   norm and update of 43.8M parameters                 281.3 us: 1.40 GB at 5.0 TB/s (torch's clipping and fused Adam: 507 us)
+//   norm and update of 36K parameters                     8.0 us: two launches
 #include "ggs_kernels.h"
 
 namespace {
@@ -40,7 +46,8 @@ __device__ __forceinline__ double block_sum(double s) {
 }
 
 // Calls f(packs, store) for a chunk, four packs a thread: all of them on their way before the first is needed where the whole
-// chunk lies inside the tensor; otherwise packs that reach over either end are filled element by element (zeros outside).  The
+// chunk lies inside the tensor; in the first and last chunk a pack that reaches over the end is filled element by element (zeros
+// outside).  The
 // 16-byte grid is the address space's: a gradient that is a view into a flat bucket starts anywhere.
 template <typename T, typename F>
 __device__ __forceinline__ void for_chunk(void* ptr, size_t numel, unsigned chunk, F&& f) {
@@ -55,13 +62,17 @@ __device__ __forceinline__ void for_chunk(void* ptr, size_t numel, unsigned chun
         for (int k = 0; k < 4; ++k) p[k] = at[k * 256];
         f(p, [&](int k, const Pack16<T>& q) { at[k * 256] = q; });
     } else {
+        const auto whole = [&](size_t e) { return (e > 0 || shift == 0) && e + VEC <= end; };
+#pragma unroll
         for (int k = 0; k < 4; ++k) {
             const size_t e = (c0 + threadIdx.x + k * 256) * VEC;
-            for (int j = 0; j < VEC; ++j) p[k].v[j] = e + j >= shift && e + j < end ? base[e + j] : (T)0.0f;
+            if (whole(e)) p[k] = *reinterpret_cast<Pack16<T>*>(base + e);
+            else for (int j = 0; j < VEC; ++j) p[k].v[j] = e + j >= shift && e + j < end ? base[e + j] : (T)0.0f;
         }
         f(p, [&](int k, const Pack16<T>& q) {
             const size_t e = (c0 + threadIdx.x + k * 256) * VEC;
-            for (int j = 0; j < VEC; ++j) if (e + j >= shift && e + j < end) base[e + j] = q.v[j];
+            if (whole(e)) *reinterpret_cast<Pack16<T>*>(base + e) = q;
+            else for (int j = 0; j < VEC; ++j) if (e + j >= shift && e + j < end) base[e + j] = q.v[j];
         });
     }
 }
@@ -88,6 +99,7 @@ __device__ __forceinline__ double chunk_squares(void* g, size_t numel, unsigned 
     return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
+// 1024 workgroups: 256 / 512 / 2048 take 63.7 / 40.9 / 39.4 us for 43.8M float gradients, 1024 take 36.4.
 __global__ __launch_bounds__(256) void k_grad_squares(GradTable t, double* partial) {
     const Finder find(t);
     const unsigned total = t.end_chunk[t.n - 1];
