@@ -33,6 +33,8 @@ struct GradTable {
     void* g[GGS_NORM_MAX_TENSORS];
 };
 
+static_assert(sizeof(GradTable) <= 4096 - 64, "the table is a kernel argument");
+
 template <typename T> struct alignas(16) Pack16 { T v[16 / sizeof(T)]; };
 
 // Sum over the 256 threads of the workgroup, the same bits in every thread.
@@ -181,6 +183,8 @@ struct ClipAdam {
     float beta2, omb1, omb2, eps;
     double beta1d, beta2d;
 };
+
+static_assert(sizeof(ClipAdam) <= 4096, "the table is a kernel argument");
 
 // ggs_adam.hip's update (torch's single-tensor Adam) with the gradient scaled first
 __device__ __forceinline__ void adam1(float& p, float g, float& m, float& v, const ClipAdam& a, float step_size, float bias2_sqrt) {

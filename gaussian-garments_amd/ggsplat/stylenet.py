@@ -10,7 +10,9 @@ What this file holds is an independent, smaller network of the same KIND, writte
   * the two autograd ops every StyleGAN2 block is made of, each expressed -- forward, backward and double backward --
     through the ONE forward op of the extension module it stands on, the way `scene/styleunet/fused_act.py:33-130` and
     `scene/styleunet/upfirdn2d.py:98-184` do it: `bias_act` (fused.fused_bias_act) and `resample2d` (upfirdn2d.upfirdn2d);
-  * plain-PyTorch twins of both (`impl="native"`), which the tests compare values and gradients against;
+  * `rms_norm`, the norm over the channels with the residual's addition (csrc/ggs_rmsnorm.hip), differentiable twice -- no part
+    of the reference's net; `StyleUNetLite(norm="rms")` uses it;
+  * plain-PyTorch twins of the three (`impl="native"`), which the tests compare values and gradients against;
   * equalised convolutions, style-modulated convolutions with demodulation, blur-filtered resampling, Haar analysis /
     synthesis -- an encoder down to 8x8, a styled decoder back up with skip connections, at the reference's channel table
     (512 features up to 64x64, then 256 / 128 / 64 / 32 -- `styleunet.py:662-672` with channel_multiplier = 2).

@@ -204,7 +204,7 @@ def adam64(p, m, v, g, k, lr, b1=0.9, b2=0.999, eps=1e-15):
     return p - step, m, v, step
 
 
-SIZES = {"one": [1], "gaussians": LISTS["gaussians"], "odd": [1, 2, 3, 5, 7, 1025, 70001], "48": [33] * 48, "many": [(k * 53) % 700 + 1 for k in range(140)],
+SIZES = {"one": [1], "gaussians": LISTS["gaussians"], "odd": [1, 2, 3, 5, 7, 1025, 70001], "48": [33] * 48, "64": [33] * 64, "65": [7] * 65, "many": [(k * 53) % 700 + 1 for k in range(140)],
          "empty_among": [0, 5, 0, 300], "large": [5_000_001, 12]}
 
 
