@@ -12,9 +12,10 @@
 // HBM-bound: the norm reads every gradient once, the scaling reads and writes it once (nothing when c = 1), the update moves
 // ggs_adam.hip's 28 bytes an element.
 // Measured (replayed from a graph, inputs of three passes in turn; a copy of 2 GiB runs at 4.9 TB/s here):
-//   norm of 43.8M float gradients (78 tensors)           36.7 us with the skipped scaling: 4.8 TB/s
-//   norm and scaling of 43.8M bf16 gradients             38.9 us: 263 MB moved, the second read from the caches
-//   norm and scaling of 6.05M float gradients (7)        11.1 us: two launches and 73 MB
+//   norm of 43.8M float gradients (78 tensors)           34.6 us: 5.1 TB/s; with the skipped scaling 36.7 us
+//   norm and scaling of 43.8M float gradients           102.8 us: 526 MB moved at 5.1 TB/s
+//   norm and scaling of 43.8M bf16 gradients             47.3 us: 263 MB moved, the second read from the caches
+//   norm and scaling of 6.05M float gradients (7)        16.0 us: two launches and 73 MB
 //   norm and update of 43.8M parameters                 281.3 us: 1.40 GB at 5.0 TB/s (torch's clipping and fused Adam: 507 us)
 //   norm and update of 36K parameters                     8.0 us: two launches
 #include "ggs_kernels.h"
