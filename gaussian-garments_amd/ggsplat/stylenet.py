@@ -204,8 +204,10 @@ def _rms_forward(x, weight, residual, eps, store):
         w32 = weight.dtype is torch.float32
     plan = (_RMS_TYPES[dtype], outer, c, inner, w32, rows)
     with on_device(dev):
-        check(lib().ggs_rms_norm_forward(plan[0], outer, c, inner, x.data_ptr(), rp, ptr(weight), w32, eps, y.data_ptr(), hp, qp,
-                                         stream_ptr(dev)), "ggs_rms_norm_forward")
+        rc = lib().ggs_rms_norm_forward(plan[0], outer, c, inner, x.data_ptr(), rp, None if weight is None else weight.data_ptr(), w32,
+                                        eps, y.data_ptr(), hp, qp, stream_ptr(dev))
+    if rc:
+        check(rc, "ggs_rms_norm_forward")
     return y, h, x, residual, weight, q, plan
 
 
@@ -245,13 +247,13 @@ class _RmsNorm(torch.autograd.Function):
 def _rms_backward(x, residual, w, q, gy, gh, plan, need_dw):
     """(dx, dw or None, gy in the kernels' order)"""
     code, outer, c, inner, w32, rows = plan
-    gy = _rms_order(gy, rows)
-    gp = rp = dw = dwp = wp = None
+    if rows or not gy.is_contiguous():
+        gy = _rms_order(gy, rows)
+    gp = dw = dwp = wp = None
     if gh is not None:
-        gh = _rms_order(gh, rows)
+        if rows or not gh.is_contiguous():
+            gh = _rms_order(gh, rows)
         gp = gh.data_ptr()
-    if residual is not None:
-        rp = residual.data_ptr()
     dx = torch.empty_like(x)
     dev, nb, L = x.device, 0, lib()
     with on_device(dev):
@@ -259,12 +261,15 @@ def _rms_backward(x, residual, w, q, gy, gh, plan, need_dw):
             dw = torch.empty_like(w)
             nb = _rms_workspace_bytes(code, outer, c, inner)
             if nb:
-                ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+                ws = q.new_empty(nb // q.element_size())              # (the accumulation type, as q)
                 dwp, wp = dw.data_ptr(), ws.data_ptr()
             else:
                 dw.zero_()                                            # no pixels
-        check(L.ggs_rms_norm_backward(code, outer, c, inner, x.data_ptr(), rp, ptr(w), w32, q.data_ptr(), gy.data_ptr(), gp,
-                                      dx.data_ptr(), dwp, wp, nb, stream_ptr(dev)), "ggs_rms_norm_backward")
+        rc = L.ggs_rms_norm_backward(code, outer, c, inner, x.data_ptr(), None if residual is None else residual.data_ptr(),
+                                     None if w is None else w.data_ptr(), w32, q.data_ptr(), gy.data_ptr(), gp, dx.data_ptr(), dwp, wp,
+                                     nb, stream_ptr(dev))
+    if rc:
+        check(rc, "ggs_rms_norm_backward")
     return dx, dw, gy
 
 
