@@ -185,30 +185,26 @@ def _rms_order(t, rows):
     return t if t.movedim(1, -1).is_contiguous() else t.movedim(1, -1).contiguous().movedim(-1, 1)
 
 
-def _rms_forward(x, weight, residual, eps, store):
-    """(y, h or None, x, residual and weight in the kernels' order, q or None, (type, outer, channels, inner, 32-bit weight, rows))"""
-    x, outer, inner, rows = _rms_layout(x)
+def _rms_forward(x, weight, residual, eps, layout, store):
+    """(y, h or None, q or None, (type, outer, channels, inner, 32-bit weight, rows)); all tensors in the kernels' order"""
+    outer, inner, rows = layout
     y = torch.empty_like(x)
     h = q = hp = rp = qp = None
     if residual is not None:
-        residual = _rms_order(residual, rows)
         h = torch.empty_like(x)
         hp, rp = h.data_ptr(), residual.data_ptr()
     dev, dtype, c = x.device, x.dtype, x.shape[1]
     if store:
         q = torch.empty(outer * inner, device=dev, dtype=torch.float64 if dtype is torch.float64 else torch.float32)
         qp = q.data_ptr()
-    w32 = False
-    if weight is not None:
-        weight = weight.contiguous()
-        w32 = weight.dtype is torch.float32
+    w32 = weight is not None and weight.dtype is torch.float32
     plan = (_RMS_TYPES[dtype], outer, c, inner, w32, rows)
     with on_device(dev):
         rc = lib().ggs_rms_norm_forward(plan[0], outer, c, inner, x.data_ptr(), rp, None if weight is None else weight.data_ptr(), w32,
                                         eps, y.data_ptr(), hp, qp, stream_ptr(dev))
     if rc:
         check(rc, "ggs_rms_norm_forward")
-    return y, h, x, residual, weight, q, plan
+    return y, h, q, plan
 
 
 @functools.lru_cache(maxsize=256)
@@ -218,8 +214,8 @@ def _rms_workspace_bytes(code, outer, c, inner):
 
 class _RmsNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, residual, eps):
-        y, h, x, residual, weight, q, ctx.plan = _rms_forward(x, weight, residual, eps, True)
+    def forward(ctx, x, weight, residual, eps, layout):
+        y, h, q, ctx.plan = _rms_forward(x, weight, residual, eps, layout, True)
         ctx.set_materialize_grads(False)
         if h is None:
             ctx.save_for_backward(x, None, weight, q)
@@ -235,13 +231,13 @@ class _RmsNorm(torch.autograd.Function):
     def backward(ctx, gy, gh=None):
         need = ctx.needs_input_grad
         if gy is None:                                                # only h was used further on
-            return gh, None, gh if need[2] else None, None
+            return gh, None, gh if need[2] else None, None, None
         x, residual, w, q = ctx.saved_tensors
         if torch.is_grad_enabled():                                   # create_graph=True
             dx, dw = _RmsNormGrad.apply(x, residual, w, q, gy, gh, ctx.plan, need[1])
         else:
             dx, dw = _rms_backward(x, residual, w, q, gy, gh, ctx.plan, need[1])[:2]
-        return dx, dw, dx if need[2] else None, None
+        return dx, dw, dx if need[2] else None, None, None
 
 
 def _rms_backward(x, residual, w, q, gy, gh, plan, need_dw):
@@ -331,10 +327,17 @@ def rms_norm(x, weight=None, residual=None, eps: float = 1e-8, impl: str = "hip"
         return _rms_norm_native(x, weight, residual, eps)
     if not x.is_cuda:
         raise RuntimeError("rms_norm: input must be a CUDA tensor")
+    # Brought into the kernels' order here, where autograd sees the copy: what _RmsNorm saves are its own inputs and outputs, which
+    # second derivatives are taken through.
+    x, outer, inner, rows = _rms_layout(x)
+    if residual is not None:
+        residual = _rms_order(residual, rows)
+    if weight is not None:
+        weight = weight.contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (residual is not None and residual.requires_grad)):
-        return _RmsNorm.apply(x, weight, residual, eps)
-    y, h = _rms_forward(x, weight, residual, eps, False)[:2]
+        return _RmsNorm.apply(x, weight, residual, eps, (outer, inner, rows))
+    y, h = _rms_forward(x, weight, residual, eps, (outer, inner, rows), False)[:2]
     return y if residual is None else (y, h)
 
 

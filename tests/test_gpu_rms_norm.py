@@ -161,6 +161,30 @@ def test_second_derivatives_against_differences():
         assert torch.autograd.gradgradcheck(lambda a, b: SN.rms_norm(a, b, eps=1e-2), (last, w), (gy,), **fast)
 
 
+def test_second_derivatives_of_strided_inputs():
+    """Inputs that the call has to bring into another order first: the second derivatives reach the tensors themselves."""
+    g = torch.Generator().manual_seed(11)
+    wide = torch.randn(2, 6, 3, 4, generator=g, dtype=torch.float64).cuda()
+    x, r = wide[..., ::2].detach().requires_grad_(), wide.flip(0)[..., 1::2].detach().requires_grad_()
+    w = torch.randn(12, generator=g, dtype=torch.float64).cuda()[::2].detach().requires_grad_()
+    gy = torch.randn(2, 6, 3, 2, generator=g, dtype=torch.float64).cuda().requires_grad_()
+    assert not x.is_contiguous() and not w.is_contiguous()
+    last = wide[..., :2].movedim(1, -1).contiguous().movedim(-1, 1).requires_grad_()
+    assert torch.autograd.gradgradcheck(lambda a, b: SN.rms_norm(a, b, eps=1e-2), (x, w), (gy,))
+    assert torch.autograd.gradgradcheck(lambda a, b, c: SN.rms_norm(a, b, residual=c, eps=1e-2), (x, w, r), (gy, gy.detach().clone().requires_grad_()))
+    assert torch.autograd.gradgradcheck(lambda a, b, c: SN.rms_norm(a, b, residual=c, eps=1e-2), (last, w, r), (gy, gy.detach().clone().requires_grad_()))
+    h, hr = wide[..., ::2].half().float().detach(), wide.flip(0)[..., 1::2].float().half().float().detach()
+    got = []
+    for impl, cast in (("hip", torch.Tensor.half), ("native", torch.Tensor.double)):              # 16 bits keep both summands
+        a, b = (cast(t) for t in (h, hr))
+        a, b = (torch.stack([t, t], -1)[..., 0].requires_grad_() for t in (a, b))
+        y, _ = SN.rms_norm(a, residual=b, eps=1e-2, impl=impl)
+        (gx,) = torch.autograd.grad((y.double() * gy).sum(), a, create_graph=True)
+        got.append(torch.autograd.grad((gx.double() * gy.flip(0)).sum(), (a, b)))
+    for p, q in zip(*got):
+        assert float((p.double() - q).norm() / q.norm()) <= 4 * HALF[torch.float16]
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
 @pytest.mark.parametrize("shape", [(40, 51), (2, 65, 9, 7), (3, 1030, 2, 2)], ids=str)
 def test_second_derivatives(shape, dtype):
