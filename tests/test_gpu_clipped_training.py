@@ -76,8 +76,12 @@ def test_captured_appearance_iteration_with_norm_and_clipping():
     assert all(torch.isfinite(p).all() for p in net_g.parameters())
 
 
-def test_captured_registration_iteration_with_clipping():
+@pytest.mark.parametrize("slack", [1.0, 0.002])
+def test_captured_registration_iteration_with_clipping(slack):
+    """slack 0.002: the first replay overflows its binning capacity, the guard voids the clipped update with the rest of the step,
+    and the step is captured again."""
     from ggsplat import inner_step as IS
+    from ggsplat import rasterizer as R
     from ggsplat.mesh_gaussian_model import MeshGaussianModel
     v, f, params, cams, gts, masks = _scene(seed=6)
     bg = torch.zeros(3, device="cuda")
@@ -90,13 +94,49 @@ def test_captured_registration_iteration_with_clipping():
         assert isinstance(m.optimizer, A.GraphAdam) and m.optimizer.max_norm == limit
         models.append(m)
     eager, graphed = models
-    step = IS.GraphedRegistrationStep(graphed, W, H, bg, opt=opt, first_frame_template=True)
+    R._cap_hint.clear()
+    step = IS.GraphedRegistrationStep(graphed, W, H, bg, opt=opt, first_frame_template=True, capacity_slack=slack)
     for ci in (0, 1, 3, 0):
         IS.registration_step(eager, cams[ci], gts[ci], masks[ci], bg, opt=opt, first_frame_template=True, fused_loss=True)
         step(cams[ci], gts[ci], masks[ci])
         a, b = float(eager.optimizer.last_grad_norm), float(graphed.optimizer.last_grad_norm)
         assert a > limit and abs(a - b) <= 1e-3 * a, (ci, a, b)
     assert graphed.optimizer.step_count == eager.optimizer.step_count == 4
+    assert step.recaptures == (0 if slack == 1.0 else 1)
     for n in ("_xyz", "_features_dc", "_opacity", "_scaling", "_rotation"):
         a, b = getattr(eager, n).detach(), getattr(graphed, n).detach()
         assert float((a - b).abs().mean()) <= 2e-4 * float(a.abs().mean()) + 1e-6, n
+
+
+def test_pipelined_and_replica_iterations_with_clipping():
+    """Two captured copies of one clipped iteration replayed alternately, and two models replayed side by side on streams of their
+    own: the same trajectories as the plain captured iteration."""
+    from ggsplat import inner_step as IS
+    from ggsplat.mesh_gaussian_model import MeshGaussianModel
+    v, f, params, cams, gts, masks = _scene(seed=6)
+    bg = torch.zeros(3, device="cuda")
+    opt = SimpleNamespace(**{**vars(IS.DEFAULT_OPT), "max_grad_norm": 1e-4})
+
+    def model():
+        m = MeshGaussianModel.from_tensors(v, f, params, sh_degree=0, device="cuda")
+        m.training_setup(opt, is_ff=True)
+        return m
+    plain, piped, r0, r1 = (model() for _ in range(4))
+    one = IS.GraphedRegistrationStep(plain, W, H, bg, opt=opt)
+    two = IS.PipelinedRegistrationStep(piped, W, H, bg, opt=opt)
+    many = IS.ReplicaRegistrationSteps([r0, r1], W, H, bg, opt=opt)
+    norms = []
+    for ci in (0, 1, 3, 0, 2):
+        one(cams[ci], gts[ci], masks[ci])
+        norms.append(float(plain.optimizer.last_grad_norm))
+        two(cams[ci], gts[ci], masks[ci])
+        many([cams[ci]] * 2, [gts[ci]] * 2, [masks[ci]] * 2)
+        for r in (r0, r1):
+            assert abs(float(r.optimizer.last_grad_norm) - norms[-1]) <= 1e-3 * norms[-1]
+    two.flush()
+    assert abs(float(piped.optimizer.last_grad_norm) - norms[-1]) <= 1e-3 * norms[-1]
+    for m in (piped, r0, r1):
+        assert m.optimizer.step_count == 5
+        for n in ("_xyz", "_features_dc", "_opacity", "_scaling", "_rotation"):
+            a, b = getattr(plain, n).detach(), getattr(m, n).detach()
+            assert float((a - b).abs().mean()) <= 2e-4 * float(a.abs().mean()) + 1e-6, n
