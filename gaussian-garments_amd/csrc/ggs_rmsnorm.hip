@@ -646,7 +646,9 @@ template <typename T> Plan plan(size_t outer, int C, size_t inner) {
         p.partials = (int)(sets < 256 ? sets : 256);          // (128 / 256 / 512: 4096 x 4096 bf16 backward 58.6 / 45.3 / 47.1 us)
         return p;
     }
-    if (C > 1024 || (size_t)C * inner > 0xffffffffu / sizeof(T)) return p;
+    // (the 32-bit byte offsets are those of a map of T and of its q, float whatever T is: one channel in 16 bits is the case where
+    // the second bound is the smaller one)
+    if (C > 1024 || (size_t)C * inner > 0xffffffffu / sizeof(T) || inner > 0xffffffffu / sizeof(float)) return p;
     p.vec = inner >= (size_t)FULL ? FULL : 1;
     // Lanes along the pixels: 16 (float) or 8 make 256 / 128 bytes of every channel, 4 make 64 and more workgroups.  Forward us of
     // 256 float channels with 4 / 8 / 16 lanes: 32 x 32 pixels 3.9 / 4.2 / 5.2, 64 x 64 6.8 / 5.5 / 6.5, 128 x 128 17.8 / 12.5 /

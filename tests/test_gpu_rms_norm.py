@@ -359,6 +359,30 @@ def test_offsets_beyond_32_bits():
         torch.cuda.empty_cache()
 
 
+def test_one_channel_with_more_pixels_than_its_q_has_32_bit_offsets_for():
+    """2^30 pixels and some, one channel in 16 bits: under 2^32 bytes of map, over 2^32 bytes of q."""
+    shape, n = (1, 1, 2 ** 15, 2 ** 15 + 8), 2 ** 15 * (2 ** 15 + 8)
+    x = torch.empty(shape, device="cuda", dtype=torch.float16)
+    flat = x.view(-1)
+    flat[:2 ** 28].normal_(generator=torch.Generator(device="cuda").manual_seed(4))
+    flat[2 ** 28:] = flat[:2 ** 28].flip(0).repeat(n // 2 ** 28 + 1)[:n - 2 ** 28]                # other values 2^30 pixels on
+    w = torch.full((1,), 1.5, device="cuda", requires_grad=True)
+    x.requires_grad_()
+    y = SN.rms_norm(x, w, eps=1.0)
+    dx, dw = torch.autograd.grad(y, (x, w), x.detach())
+    rows = lambda t, k: t.detach()[:, :, k:k + 1]                                 # noqa: E731
+    for k in (0, 1, 2 ** 14, 2 ** 15 - 9, 2 ** 15 - 8, 2 ** 15 - 7, 2 ** 15 - 1):         # (pixel 2^30 lies in row 2^15 - 8)
+        ref, size = reference(rows(x, k), w, None, rows(x, k), None, eps=1.0)
+        for name, v in (("y", y), ("dx", dx)):
+            held(name, rows(v, k), ref[name], size[name], 1, 9, torch.float16)
+    want = 0.0
+    for part in flat.detach().split(2 ** 26):
+        d = part.double()
+        want += float((d * d / (d * d + 1).sqrt()).sum())
+    # (every term is positive: a thread adds up to 2^30 / 2^14 + 1 = 65537 of them one after the other, half a float step each)
+    assert abs(float(dw) - want) <= want * 65600 * 2.0 ** -24, (float(dw), want)
+
+
 @pytest.mark.parametrize("shape,dtype", [((2 ** 29 + 5, 1), torch.float16), ((2 ** 25 + 3, 1, 3), torch.float16), ((2 ** 23 + 3, 1), torch.float64),
                                          ((2 ** 23 + 3, 1, 2), torch.float64)], ids=str)
 def test_more_work_than_one_launch_takes(shape, dtype):

@@ -114,6 +114,17 @@ def test_c_entry_points_check_before_any_launch():
     assert "NULL" in two(0, 1000, 64, 7, one, None, one, 0, one, None, one, None, one, one, one, one, nb, None)[1]
 
 
+def test_which_maps_the_one_pass_kernels_take():
+    """Their workspace is a row of partials a workgroup (8192 / waves at most), that of the two-pass kernels at most 64 rows: a map
+    whose elements or whose float q lie beyond 32-bit byte offsets goes to the latter."""
+    L = _lib.lib()
+    rows = lambda code, c, inner: L.ggs_rms_norm_workspace_bytes(code, 1, c, inner) // (4 * c)                # noqa: E731
+    for code in (1, 3):                                                          # 16 bits: 2 bytes an element, 4 a q
+        assert rows(code, 1, 2 ** 30 - 1) == 8192 and rows(code, 1, 2 ** 30) == 64 and rows(code, 1, 2 ** 31 - 1) == 64
+        assert rows(code, 2, 2 ** 30 - 1) == 8192 and rows(code, 2, 2 ** 30) == 64
+    assert rows(0, 1, 2 ** 30 - 1) == 8192 and rows(0, 1, 2 ** 30) == 64
+
+
 def test_training_setup_clips_only_with_the_gpu_optimiser():
     from types import SimpleNamespace
     from ggsplat.inner_step import DEFAULT_OPT
