@@ -37,6 +37,7 @@ os.environ.setdefault("MIOPEN_DEBUG_CONV_IMPLICIT_GEMM_ASM_BWD_GTC_XDLOPS_NHWC",
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from ._lib import check, lib, on_device, ptr, stream_ptr
 
@@ -163,8 +164,8 @@ _RMS_TYPES = {torch.float32: 0, torch.float16: 1, torch.float64: 2, torch.bfloat
 
 
 def _rms_layout(x):
-    """(x as the kernels read it, outer, inner, whether channels are innermost): channels-last maps and whatever else keeps the
-    channels of a pixel together are rows, the rest is [B][C][pixels]."""
+    """(x as the kernels read it, (outer, channels, inner, whether channels are innermost)): channels-last maps and whatever else
+    keeps the channels of a pixel together are rows, the rest is [B][C][pixels]."""
     if x.is_contiguous():
         rows = False
     else:
@@ -175,7 +176,7 @@ def _rms_layout(x):
     inner = 1
     for s in shape[2:]:
         inner *= s
-    return (x, shape[0] * inner, 1, True) if rows else (x, shape[0], inner, False)
+    return x, ((shape[0] * inner, shape[1], 1, True) if rows else (shape[0], shape[1], inner, False))
 
 
 def _rms_order(t, rows):
@@ -187,13 +188,13 @@ def _rms_order(t, rows):
 
 def _rms_forward(x, weight, residual, eps, layout, store):
     """(y, h or None, q or None, (type, outer, channels, inner, 32-bit weight, rows)); all tensors in the kernels' order"""
-    outer, inner, rows = layout
+    outer, c, inner, rows = layout
     y = torch.empty_like(x)
     h = q = hp = rp = qp = None
     if residual is not None:
         h = torch.empty_like(x)
         hp, rp = h.data_ptr(), residual.data_ptr()
-    dev, dtype, c = x.device, x.dtype, x.shape[1]
+    dev, dtype = x.device, x.dtype
     if store:
         q = torch.empty(outer * inner, device=dev, dtype=torch.float64 if dtype is torch.float64 else torch.float32)
         qp = q.data_ptr()
@@ -215,6 +216,13 @@ def _rms_workspace_bytes(code, outer, c, inner):
 class _RmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps, layout):
+        if layout is None:                    # recorded by torch.jit.trace: every run may bring tensors of other shapes
+            _rms_check(x, weight, residual)
+            if not x.is_cuda:
+                raise RuntimeError("rms_norm: input must be a CUDA tensor")
+            x, weight, residual = (None if t is None else t.contiguous() for t in (x, weight, residual))
+            shape = [int(s) for s in x.shape]
+            layout = (shape[0], shape[1], math.prod(shape[2:]), False)
         y, h, q, ctx.plan = _rms_forward(x, weight, residual, eps, layout, True)
         ctx.set_materialize_grads(False)
         if h is None:
@@ -305,12 +313,7 @@ class _RmsNormGrad(torch.autograd.Function):
         return dh, dh if need[1] else None, dw, None, dgy if need[4] else None, v if need[5] else None, None, None
 
 
-def rms_norm(x, weight=None, residual=None, eps: float = 1e-8, impl: str = "hip"):
-    """y = weight[channel] * h / sqrt(mean over the channels of h^2 + eps), h = x (+ residual), for x [B, C, ...] (every pixel of a
-    feature map by itself; [rows, C]: every row).  Returns y, or (y, h) with a residual -- h is the sum to carry on.
-    x, residual: float32 / float16 / bfloat16 / float64, the same shape; weight [C]: x's type or float32; contiguous and
-    channels-last maps are taken as they are.  The norm is that of the unrounded sum; sums are in float (double for float64).
-    Differentiable twice (second derivatives are not differentiable again)."""
+def _rms_check(x, weight, residual):
     shape, dtype = x.shape, x.dtype
     if len(shape) < 2 or shape[1] == 0:
         raise ValueError(f"rms_norm: x must be [B, C, ...] with C > 0, got {tuple(shape)}")
@@ -320,6 +323,15 @@ def rms_norm(x, weight=None, residual=None, eps: float = 1e-8, impl: str = "hip"
         raise ValueError("rms_norm: residual must have x's shape, type and device")
     if weight is not None and (weight.shape != shape[1:2] or weight.dtype not in (dtype, torch.float32) or weight.device != x.device):
         raise ValueError("rms_norm: weight must be [C], of x's type or float32, on x's device")
+
+
+def rms_norm(x, weight=None, residual=None, eps: float = 1e-8, impl: str = "hip"):
+    """y = weight[channel] * h / sqrt(mean over the channels of h^2 + eps), h = x (+ residual), for x [B, C, ...] (every pixel of a
+    feature map by itself; [rows, C]: every row).  Returns y, or (y, h) with a residual -- h is the sum to carry on.
+    x, residual: float32 / float16 / bfloat16 / float64, the same shape; weight [C]: x's type or float32; contiguous and
+    channels-last maps are taken as they are.  The norm is that of the unrounded sum; sums are in float (double for float64).
+    Differentiable twice (second derivatives are not differentiable again), not in forward mode; torch.jit.trace records a call."""
+    _rms_check(x, weight, residual)
     eps = float(eps)
     if not (eps > 0.0 and math.isfinite(eps)):
         raise ValueError("rms_norm: eps must be positive")
@@ -327,17 +339,22 @@ def rms_norm(x, weight=None, residual=None, eps: float = 1e-8, impl: str = "hip"
         return _rms_norm_native(x, weight, residual, eps)
     if not x.is_cuda:
         raise RuntimeError("rms_norm: input must be a CUDA tensor")
+    if torch.jit.is_tracing():
+        return _RmsNorm.apply(x.contiguous(), None if weight is None else weight.contiguous(),
+                              None if residual is None else residual.contiguous(), eps, None)
     # Brought into the kernels' order here, where autograd sees the copy: what _RmsNorm saves are its own inputs and outputs, which
     # second derivatives are taken through.
-    x, outer, inner, rows = _rms_layout(x)
+    x, layout = _rms_layout(x)
     if residual is not None:
-        residual = _rms_order(residual, rows)
+        residual = _rms_order(residual, layout[3])
     if weight is not None:
         weight = weight.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (residual is not None and residual.requires_grad)):
-        return _RmsNorm.apply(x, weight, residual, eps, (outer, inner, rows))
-    y, h = _rms_forward(x, weight, residual, eps, (outer, inner, rows), False)[:2]
+    # The C call alone where nothing but autograd's backward mode could ask for the Function, and does not: a forward-mode level
+    # that is open (its tangents need no requires_grad) goes through it and is refused there.
+    if forward_ad._current_level >= 0 or torch.is_grad_enabled() and (
+            x.requires_grad or (weight is not None and weight.requires_grad) or (residual is not None and residual.requires_grad)):
+        return _RmsNorm.apply(x, weight, residual, eps, layout)
+    y, h = _rms_forward(x, weight, residual, eps, layout, False)[:2]
     return y if residual is None else (y, h)
 
 

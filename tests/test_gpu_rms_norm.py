@@ -414,3 +414,24 @@ def test_gradients_of_two_leaves_do_not_share_memory():
     y, h = SN.rms_norm(x, w, residual=r)
     torch.autograd.backward((y, h), (gy, gh))
     assert torch.equal(x.grad, r.grad) and x.grad.data_ptr() != r.grad.data_ptr()
+
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+def test_traced_calls():
+    """torch.jit.trace of calls with and without a gradient: run on tensors of other sizes, layouts and values, and differentiated."""
+    x, w, r, gy, gh = tensors((2, 12, 5, 5), torch.float32, "same", True)
+    with torch.no_grad():
+        one = torch.jit.trace(lambda t: SN.rms_norm(t), (x,))
+    two = torch.jit.trace(lambda a, b, c: SN.rms_norm(a, c, residual=b, eps=EPS), (x.requires_grad_(), r, w))
+    for shape in ((2, 12, 5, 5), (1, 12, 3, 70), (5, 40, 1, 1), (0, 12, 5, 5)):
+        x, w, r, gy, gh = tensors(shape, torch.float32, "same", True, seed=1)
+        assert torch.equal(one(x), SN.rms_norm(x))
+        xl = x.to(memory_format=torch.channels_last)
+        ref, size = reference(xl, None, None, None, None)
+        held("y", one(xl), ref["y"], size["y"], shape[1], 1, torch.float32)
+        want = passes(x, w, r, gy, gh)
+        leaves = [t.detach().requires_grad_() for t in (x, r, w)]
+        y, h = two(*leaves)
+        dx, dr, dw = torch.autograd.grad((y, h), leaves, (gy, gh))
+        for k, v in (("y", y), ("h", h), ("dx", dx), ("dr", dr), ("dw", dw)):
+            assert torch.equal(v, want[k]), k

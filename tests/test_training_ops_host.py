@@ -1,7 +1,9 @@
 """Host side of the training-step operators (rms_norm, grad_norm / clip_grad_norm_, GraphAdam(max_norm)): what they refuse, and
 the argument checks of their C entry points.  Nothing is launched."""
+import contextlib
 import ctypes as C
 
+import numpy as np
 import pytest
 import torch
 
@@ -38,6 +40,57 @@ def test_rms_norm_native_is_the_formula():
     s = 12.5 ** 0.5
     assert torch.equal(h, x + r) and torch.allclose(y, torch.tensor([[3 / s, 8 / s], [1.0, -2.0]], dtype=torch.float64))
     assert torch.equal(SN.rms_norm(torch.zeros(1, 5), impl="native"), torch.zeros(1, 5))
+
+
+@pytest.fixture
+def norm_on_the_host(monkeypatch):
+    """rms_norm's C call computed on the host (float, channels-first), for what happens around it."""
+    class Lib:
+        @staticmethod
+        def ggs_rms_norm_forward(code, outer, c, inner, x, r, w, w32, eps, y, h, q, stream):
+            view = lambda at, *n: None if at is None else np.ctypeslib.as_array((C.c_float * int(np.prod(n))).from_address(at)).reshape(n)    # noqa: E731
+            assert code == 0 and all(type(n) is int for n in (outer, c, inner))
+            s = view(x, outer, c, inner) + (0 if r is None else view(r, outer, c, inner))
+            inv = 1 / np.sqrt((s * s).mean(1, keepdims=True) + eps)
+            view(y, outer, c, inner)[:] = s * inv * (1 if w is None else view(w, c, 1))
+            if h is not None:
+                view(h, outer, c, inner)[:] = s
+            if q is not None:
+                view(q, outer, 1, inner)[:] = inv
+            return 0
+    monkeypatch.setattr(SN, "lib", lambda: Lib)
+    monkeypatch.setattr(SN, "on_device", lambda dev: contextlib.nullcontext())
+    monkeypatch.setattr(SN, "stream_ptr", lambda dev: None)
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda t: True))
+
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+def test_rms_norm_in_a_trace_is_a_call(norm_on_the_host):
+    x, r, w = torch.randn(3, 5, 2), torch.randn(3, 5, 2), torch.rand(5)
+    with torch.no_grad():
+        one = torch.jit.trace(lambda t: SN.rms_norm(t) + 1, (x,))                # (traced twice and compared)
+    two = torch.jit.trace(lambda a, b, c: SN.rms_norm(a, c, residual=b), (x, r, w))
+    for shape in ((3, 5, 2), (0, 5, 2), (1, 5, 7), (4, 9, 1)):                   # other sizes than the traced ones
+        x, r, w = torch.randn(shape), torch.randn(shape), torch.rand(shape[1])
+        assert torch.allclose(one(x), SN.rms_norm(x, impl="native") + 1, rtol=1e-5, atol=1e-6)
+        for a, b in zip(two(x, r, w), SN.rms_norm(x, w, residual=r, impl="native")):
+            assert torch.allclose(a, b, rtol=1e-5, atol=1e-6)
+    t = torch.randn(2, 4, 3).transpose(0, 1)
+    assert torch.allclose(one(t), SN.rms_norm(t, impl="native") + 1, rtol=1e-5, atol=1e-6)
+    for bad in ((x, r[:1], w), (x, r, w[:2]), (x, r.double(), w), (x[0, 0], r[0, 0], w)):      # checked in every run
+        with pytest.raises(Exception, match="rms_norm"):
+            two(*bad)
+
+
+def test_rms_norm_refuses_forward_mode(norm_on_the_host):
+    from torch.autograd import forward_ad as fw
+    x, t = torch.randn(3, 5), torch.randn(3, 5)
+    with fw.dual_level():
+        for args in ((fw.make_dual(x, t),), (x, fw.make_dual(t[0], t[0])), (x, None, fw.make_dual(x, t))):
+            with torch.no_grad(), pytest.raises(NotImplementedError):
+                SN.rms_norm(*args)
+        assert torch.allclose(SN.rms_norm(x), SN.rms_norm(x, impl="native"), rtol=1e-5, atol=1e-6)      # no tangent: as ever
+        assert fw.unpack_dual(SN.rms_norm(fw.make_dual(x, t), impl="native")).tangent is not None
 
 
 def test_norm_of_the_network_adds_only_its_gains():
