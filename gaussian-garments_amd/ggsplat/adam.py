@@ -328,7 +328,7 @@ class GraphAdam:
             lr += 4
         if self.max_norm is not None:
             self._clipped_step(L, numel, cols, tick, gp, stream)
-            increment_version(params)
+            increment_version(params)              # written in place: saved tensors and cached bindings of them are void
             return
         for k in range(0, len(numel), 16):                     # one launch per 16 tensors
             sizes = numel[k:k + 16]
@@ -338,6 +338,7 @@ class GraphAdam:
             fn = L.ggs_adam_tick_step_multi if tick else L.ggs_adam_step_multi
             check(fn(n, (C.c_size_t * n)(*sizes), *chunk, b1, b2, self.eps, gp, stream),
                   "ggs_adam_tick_step_multi" if tick else "ggs_adam_step_multi")
+        increment_version(params)
 
     def _clipped_step(self, L, numel, cols, tick: bool, gp, stream) -> None:
         n = len(numel)

@@ -368,3 +368,32 @@ def test_writes_in_place_are_seen_by_autograd():
     opt.step()
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+@pytest.mark.parametrize("max_norm", [None, 1.0], ids=str)
+def test_every_step_is_seen_by_autograd_and_by_cached_bindings(max_norm):
+    """With and without clipping: a tensor saved before the step, and the mesh binding that a model keeps between its getters."""
+    from types import SimpleNamespace
+    from ggsplat.inner_step import DEFAULT_OPT
+    from ggsplat.mesh_gaussian_model import MeshGaussianModel
+    from test_gpu_graph_step import _scene
+    p = torch.nn.Parameter(torch.ones(8, device="cuda"))
+    unused = torch.nn.Parameter(torch.ones(8, device="cuda"))
+    opt = A.GraphAdam([p, unused], lr=1e-2, max_norm=max_norm)
+    y, z = (p * p).sum(), (unused * unused).sum()
+    p.grad = torch.ones_like(p)
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    z.backward()                                                                 # had no gradient, was not written
+    v, f, params, _, _, _ = _scene(seed=6)
+    m = MeshGaussianModel.from_tensors(v, f, params, sh_degree=0, device="cuda")
+    m.training_setup(SimpleNamespace(**{**vars(DEFAULT_OPT), "max_grad_norm": max_norm}), is_ff=True)
+    for q, get in ((m._xyz, lambda: m.get_xyz), (m._scaling, lambda: m.get_scaling), (m._rotation, lambda: m.get_rotation)):
+        before = get().detach().clone()
+        q.grad = torch.randn(q.shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+        m.optimizer.step()
+        m.optimizer.zero_grad()
+        got = get().detach().clone()
+        m.update_face_coor()
+        assert torch.equal(got, get()) and not torch.equal(got, before)
