@@ -10,6 +10,7 @@ from typing import List, Callable, Dict, Optional
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.graph import increment_version
 
 from . import rasterizer as R
 from .adam import GraphAdam
@@ -497,6 +498,13 @@ class GraphedRegistrationStep:
             self._capture()
             # the capture itself does not execute anything: the caller replays
 
+    def _replay(self):
+        self.graph.replay()
+        # a replay writes the parameters where autograd does not see it: cached bindings and saved tensors of them are void
+        opt = getattr(self, "optimizer", None) or self.g.optimizer
+        if opt is not None:
+            increment_version([p for group in opt.param_groups for p in group["params"]])
+
     # ---- split form of __call__ for PipelinedRegistrationStep: queue an iteration / read its result later -----------------
     def launch(self, cam, gt_image, mask=None) -> None:
         """Queue one iteration on the current stream WITHOUT waiting for it: parameter block, graph replay, result read-back
@@ -504,7 +512,7 @@ class GraphedRegistrationStep:
         self._last_args = (cam, gt_image, mask)
         self._load(cam, gt_image, mask)
         self._ready_graph()
-        self.graph.replay()
+        self._replay()
         if not self._out_map:
             self._out_host.copy_(self._out, non_blocking=True)
         if getattr(self, "_done", None) is None:
@@ -526,7 +534,7 @@ class GraphedRegistrationStep:
         self._load(cam, gt_image, mask)
         self._ready_graph()
         while True:
-            self.graph.replay()
+            self._replay()
             if not self._out_map:
                 self._out_host.copy_(self._out, non_blocking=True)
             torch.cuda.current_stream().synchronize()

@@ -397,3 +397,24 @@ def test_every_step_is_seen_by_autograd_and_by_cached_bindings(max_norm):
         got = get().detach().clone()
         m.update_face_coor()
         assert torch.equal(got, get()) and not torch.equal(got, before)
+
+
+@pytest.mark.parametrize("lean", [True, False])
+def test_a_replayed_step_is_seen_by_cached_bindings(lean):
+    from ggsplat.inner_step import DEFAULT_OPT, GraphedRegistrationStep
+    from ggsplat.mesh_gaussian_model import MeshGaussianModel
+    from test_gpu_graph_step import H, W, _scene
+    v, f, params, cams, gts, masks = _scene(seed=6)
+    m = MeshGaussianModel.from_tensors(v, f, params, sh_degree=0, device="cuda")
+    m.training_setup(DEFAULT_OPT, is_ff=True)
+    step = GraphedRegistrationStep(m, W, H, torch.zeros(3, device="cuda"), opt=DEFAULT_OPT, lean=lean)
+    for ci in (0, 1, 3):                                                         # the capture, then replays alone
+        before = m.get_xyz.detach().clone()
+        step(cams[ci], gts[ci], masks[ci])
+        got = m.get_xyz.detach().clone()
+        m.update_face_coor()
+        assert torch.equal(got, m.get_xyz) and not torch.equal(got, before), ci
+    y = (m._xyz * m._xyz).sum()
+    step(cams[0], gts[0], masks[0])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
