@@ -133,7 +133,9 @@ __device__ __forceinline__ float clip_factor(double norm, double max_norm) {
     return c > 1.0 ? 1.0f : (float)c;
 }
 
-__global__ __launch_bounds__(256) void k_grad_norm(const double* partial, int n, float* norm) {
+// guard (NULL: none): a word that voids the write
+__global__ __launch_bounds__(256) void k_grad_norm(const double* partial, int n, float* norm, const unsigned long long* guard) {
+    if (guard && *guard) return;
     const double d = norm_of(partial, n);
     if (threadIdx.x == 0) *norm = (float)d;
 }
@@ -313,8 +315,9 @@ int launch_squares(const char* who, int n, const size_t* numel, const void* cons
     return GGS_OK;
 }
 
-int launch_norm(const char* who, const void* workspace, int n_partial, float* norm, hipStream_t s) {
-    hipLaunchKernelGGL(k_grad_norm, dim3(1), dim3(256), 0, s, static_cast<const double*>(workspace), n_partial, norm);
+int launch_norm(const char* who, const void* workspace, int n_partial, float* norm, const void* guard, hipStream_t s) {
+    hipLaunchKernelGGL(k_grad_norm, dim3(1), dim3(256), 0, s, static_cast<const double*>(workspace), n_partial, norm,
+                       static_cast<const unsigned long long*>(guard));
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return ggs_fail_(GGS_ERR_HIP, "%s: launch failed: %s", who, hipGetErrorString(e));
     return GGS_OK;
@@ -335,7 +338,7 @@ int ggs_grad_norm(int n_tensors, const size_t* numel, const void* const* grads, 
     if (rc != GGS_OK) return rc;
     if (!norm) return ggs_fail_(GGS_ERR_ARG, "ggs_grad_norm: NULL norm");
     rc = launch_squares("ggs_grad_norm", n_tensors, numel, grads, dtypes, workspace, workspace_bytes, &n_partial, (hipStream_t)stream);
-    return rc != GGS_OK ? rc : launch_norm("ggs_grad_norm", workspace, n_partial, norm, (hipStream_t)stream);
+    return rc != GGS_OK ? rc : launch_norm("ggs_grad_norm", workspace, n_partial, norm, nullptr, (hipStream_t)stream);
 }
 
 int ggs_grad_clip(int n_tensors, const size_t* numel, void* const* grads, const int* dtypes, double max_norm, float* norm,
@@ -348,7 +351,7 @@ int ggs_grad_clip(int n_tensors, const size_t* numel, void* const* grads, const 
     hipStream_t s = (hipStream_t)stream;
     rc = launch_squares("ggs_grad_clip", n_tensors, numel, grads, dtypes, workspace, workspace_bytes, &n_partial, s);
     if (rc != GGS_OK) return rc;
-    if (n_partial == 0) return launch_norm("ggs_grad_clip", workspace, 0, norm, s);
+    if (n_partial == 0) return launch_norm("ggs_grad_clip", workspace, 0, norm, nullptr, s);
     GradTable t;
     bool first = true;
     for (int i = 0; next_table(t, i, n_tensors, numel, grads, dtypes); first = false) {
@@ -384,7 +387,7 @@ int ggs_adam_clip_step(int n_tensors, const size_t* numel, float* const* params,
     hipStream_t s = (hipStream_t)stream;
     rc = launch_squares("ggs_adam_clip_step", n_tensors, numel, gv, nullptr, workspace, workspace_bytes, &n_partial, s);
     if (rc != GGS_OK) return rc;
-    if (n_partial == 0) return launch_norm("ggs_adam_clip_step", workspace, 0, norm, s);
+    if (n_partial == 0) return launch_norm("ggs_adam_clip_step", workspace, 0, norm, guard, s);
     ClipAdam a;
     a.tick = tick; a.guard = static_cast<const unsigned long long*>(guard);
     a.partial = static_cast<const double*>(workspace); a.n_partial = n_partial; a.max_norm = max_norm; a.norm = norm;

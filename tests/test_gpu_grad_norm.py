@@ -418,3 +418,18 @@ def test_a_replayed_step_is_seen_by_cached_bindings(lean):
     step(cams[0], gts[0], masks[0])
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+def test_a_void_step_without_gradients_keeps_the_norm():
+    p = torch.nn.Parameter(torch.zeros(2, device="cuda"))
+    opt = A.GraphAdam([p], lr=1e-2, max_norm=1.0)
+    p.grad = torch.tensor([3.0, 4.0], device="cuda")
+    opt.step()
+    guard = torch.ones(1, dtype=torch.int64, device="cuda")
+    for void in (p.grad, None):
+        p.grad = void
+        opt.step(guard=guard)
+        assert float(opt.last_grad_norm) == 5.0
+    guard.zero_()
+    opt.step(guard=guard)
+    assert float(opt.last_grad_norm) == 0.0
