@@ -64,7 +64,7 @@ class _GradList:
             at = g.get_device()
             if at < 0:
                 raise RuntimeError("ggsplat: gradient norms run on the GPU only (no CPU path in the product)")
-            if g.requires_grad:
+            if g.requires_grad and g.is_leaf:      # (gradients of backward(create_graph=True) require grad, but are no leaves)
                 raise ValueError("ggsplat: pass the gradients ([p.grad for p in params]), not the parameters")
             if g.layout is not torch.strided:
                 raise TypeError("ggsplat: sparse gradients are not supported")
@@ -117,7 +117,7 @@ class _GradList:
 def grad_norm(grads) -> torch.Tensor:
     """The length of `grads` (a tensor, or tensors of float32 / float16 / bfloat16 in any mixture; None entries are skipped) as
     ONE vector: sqrt(sum of all squares), a 0-dim float32 tensor on their device, 0 for no gradients at all.  Asynchronous on the
-    current stream, capturable; sums in double, the same bits on every run."""
+    current stream, capturable; sums in double, the same bits on every run.  Not differentiable."""
     gl = _GradList(grads, False)
     if gl.device is None:
         return torch.tensor(0.0)
@@ -133,7 +133,8 @@ def clip_grad_norm_(grads, max_norm: float, error_if_nonfinite: bool = False) ->
     """Scales every gradient in place by min(1, max_norm / (N + 1e-6)) and returns N = grad_norm(grads), as
     torch.nn.utils.clip_grad_norm_ does for the gradients of its parameters (norm_type 2).  A NaN norm makes every gradient NaN,
     an infinite one zero (NaN where it was infinite); `error_if_nonfinite` raises instead and leaves the gradients as they were,
-    which needs the norm on the host: a synchronisation, refused inside a capture.  No two gradients may overlap in memory."""
+    which needs the norm on the host: a synchronisation, refused inside a capture.  No two gradients may overlap in memory.  Gradients
+    that were computed with create_graph=True are scaled as plain values."""
     max_norm = _checked_max_norm(max_norm)
     gl = _GradList(grads, True)
     if gl.device is None:

@@ -433,3 +433,22 @@ def test_a_void_step_without_gradients_keeps_the_norm():
     guard.zero_()
     opt.step(guard=guard)
     assert float(opt.last_grad_norm) == 0.0
+
+
+def test_gradients_that_were_computed_with_a_graph():
+    p, q = (torch.nn.Parameter(torch.linspace(0.5, 2.0, n, device="cuda")) for n in (7, 30))
+    with pytest.warns(UserWarning, match="create_graph"):
+        ((p ** 3).sum() + (q ** 4).sum()).backward(create_graph=True)
+    gs = [p.grad, q.grad]
+    assert all(g.requires_grad for g in gs)
+    keep = [g.detach().clone() for g in gs]
+    total = A.grad_norm(gs)
+    same_norm(total, keep)
+    assert not total.requires_grad
+    assert torch.equal(A.clip_grad_norm_(gs, 1.0), total)
+    A.clip_grad_norm_(keep, 1.0)
+    assert all(torch.equal(g, k) for g, k in zip(gs, keep))
+    opt = A.GraphAdam([p, q], lr=1e-2, max_norm=0.5)
+    opt.step()
+    same_norm(opt.last_grad_norm, keep)
+    p.grad = q.grad = None
