@@ -22,6 +22,7 @@ import math
 from typing import Dict, Iterable, List, Optional
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.graph import increment_version
 
 from ._lib import check, lib, on_device, ptr, stream_ptr
@@ -54,7 +55,10 @@ class _GradList:
     matter to the norm, so any dense layout is read in place; a strided one is read (and written back) through a copy."""
 
     def __init__(self, grads, in_place: bool):
+        if torch.jit.is_tracing():                 # the trace would hold the allocation of the norm and not what fills it
+            raise RuntimeError("ggsplat: gradient norms cannot be recorded by torch.jit.trace")
         self.device, self.copies, self.keep = None, [], []
+        dual = forward_ad._current_level >= 0
         index, numel, ptrs, types, ends = None, [], [], [], []
         for g in ([grads] if isinstance(grads, torch.Tensor) else grads):
             if g is None:
@@ -66,6 +70,8 @@ class _GradList:
                 raise RuntimeError("ggsplat: gradient norms run on the GPU only (no CPU path in the product)")
             if g.requires_grad and g.is_leaf:      # (gradients of backward(create_graph=True) require grad, but are no leaves)
                 raise ValueError("ggsplat: pass the gradients ([p.grad for p in params]), not the parameters")
+            if dual and forward_ad.unpack_dual(g).tangent is not None:
+                raise NotImplementedError("ggsplat: gradient norms have no forward-mode derivative")
             if g.layout is not torch.strided:
                 raise TypeError("ggsplat: sparse gradients are not supported")
             if at != index:

@@ -452,3 +452,16 @@ def test_gradients_that_were_computed_with_a_graph():
     opt.step()
     same_norm(opt.last_grad_norm, keep)
     p.grad = q.grad = None
+
+
+def test_traces_and_forward_mode_are_refused():
+    from torch.autograd import forward_ad as fw
+    g = torch.tensor([3.0, 4.0], device="cuda")
+    for fn in (A.grad_norm, lambda t: A.clip_grad_norm_(t, 1.0)):
+        with pytest.raises(RuntimeError, match="trace"):
+            torch.jit.trace(fn, (g,), check_trace=False)
+        with fw.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+            fn([g, fw.make_dual(g, g)])
+    assert torch.equal(g, torch.tensor([3.0, 4.0], device="cuda"))
+    with fw.dual_level():
+        assert float(A.grad_norm([g])) == 5.0                                    # a level that is open, no tangent

@@ -113,6 +113,12 @@ def test_gradient_list_refusals():
     assert float(A.clip_grad_norm_([], float("inf"))) == 0.0
 
 
+def test_gradient_norms_are_not_traced():
+    for fn in (A.grad_norm, lambda g: A.clip_grad_norm_(g, 1.0)):
+        with pytest.raises(RuntimeError, match="trace"):
+            torch.jit.trace(lambda g: fn([]) + g, (torch.zeros(3),), check_trace=False)
+
+
 def test_span_of_layouts():
     t = torch.zeros(4, 6, 5)
     assert A._span(t) == (120, True, False) and A._span(t.permute(2, 0, 1)) == (120, True, False)
