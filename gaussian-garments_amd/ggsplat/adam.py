@@ -122,11 +122,11 @@ class _GradList:
 @torch.no_grad()
 def grad_norm(grads) -> torch.Tensor:
     """The length of `grads` (a tensor, or tensors of float32 / float16 / bfloat16 in any mixture; None entries are skipped) as
-    ONE vector: sqrt(sum of all squares), a 0-dim float32 tensor on their device, 0 for no gradients at all.  Asynchronous on the
+    ONE vector: sqrt(sum of all squares), a 0-dim float32 tensor on their device; 0 for no gradients at all, on the default device.  Asynchronous on the
     current stream, capturable; sums in double, the same bits on every run.  Not differentiable."""
     gl = _GradList(grads, False)
     if gl.device is None:
-        return torch.tensor(0.0)
+        return torch.zeros((), dtype=torch.float32)
     with on_device(gl.device):
         norm, nb, ws = gl.buffers()
         check(lib().ggs_grad_norm(gl.n, gl.numel, gl.ptrs, gl.types, norm.data_ptr(), ptr(ws), nb, stream_ptr(gl.device)),
@@ -144,7 +144,7 @@ def clip_grad_norm_(grads, max_norm: float, error_if_nonfinite: bool = False) ->
     max_norm = _checked_max_norm(max_norm)
     gl = _GradList(grads, True)
     if gl.device is None:
-        return torch.tensor(0.0)
+        return torch.zeros((), dtype=torch.float32)
     if error_if_nonfinite:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("ggsplat: error_if_nonfinite needs the norm on the host and cannot be captured")

@@ -113,6 +113,16 @@ def test_gradient_list_refusals():
     assert float(A.clip_grad_norm_([], float("inf"))) == 0.0
 
 
+def test_norm_of_nothing_is_float32():
+    keep = torch.get_default_dtype()
+    try:
+        torch.set_default_dtype(torch.float64)
+        for n in (A.grad_norm([]), A.clip_grad_norm_([None], 1.0)):
+            assert n.dtype is torch.float32 and n.shape == () and float(n) == 0.0
+    finally:
+        torch.set_default_dtype(keep)
+
+
 def test_gradient_norms_are_not_traced():
     for fn in (A.grad_norm, lambda g: A.clip_grad_norm_(g, 1.0)):
         with pytest.raises(RuntimeError, match="trace"):
