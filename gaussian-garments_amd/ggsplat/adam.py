@@ -106,7 +106,8 @@ class _GradList:
             last = 0
             for lo, hi in ends:
                 if lo < last:
-                    raise ValueError("ggsplat: two of the gradients overlap in memory (the same one listed twice?)")
+                    raise ValueError("ggsplat: the memory of two gradients overlaps, from first to last element (the same one listed "
+                                     "twice, or strided views that interleave: clip the tensor that they are views of)")
                 last = hi
         self.n = n = len(numel)
         self.numel, self.ptrs, self.types = (C.c_size_t * n)(*numel), (C.c_void_p * n)(*ptrs), (C.c_int * n)(*types)
@@ -122,8 +123,8 @@ class _GradList:
 @torch.no_grad()
 def grad_norm(grads) -> torch.Tensor:
     """The length of `grads` (a tensor, or tensors of float32 / float16 / bfloat16 in any mixture; None entries are skipped) as
-    ONE vector: sqrt(sum of all squares), a 0-dim float32 tensor on their device; 0 for no gradients at all, on the default device.  Asynchronous on the
-    current stream, capturable; sums in double, the same bits on every run.  Not differentiable."""
+    ONE vector: sqrt(sum of all squares), a 0-dim float32 tensor on their device (0 on the default device for no gradients at
+    all).  Asynchronous on the current stream, capturable; sums in double, the same bits on every run.  Not differentiable."""
     gl = _GradList(grads, False)
     if gl.device is None:
         return torch.zeros((), dtype=torch.float32)
@@ -139,8 +140,9 @@ def clip_grad_norm_(grads, max_norm: float, error_if_nonfinite: bool = False) ->
     """Scales every gradient in place by min(1, max_norm / (N + 1e-6)) and returns N = grad_norm(grads), as
     torch.nn.utils.clip_grad_norm_ does for the gradients of its parameters (norm_type 2).  A NaN norm makes every gradient NaN,
     an infinite one zero (NaN where it was infinite); `error_if_nonfinite` raises instead and leaves the gradients as they were,
-    which needs the norm on the host: a synchronisation, refused inside a capture.  No two gradients may overlap in memory.  Gradients
-    that were computed with create_graph=True are scaled as plain values."""
+    which needs the norm on the host: a synchronisation, refused inside a capture.  No two gradients may overlap in memory,
+    first to last element: strided views that interleave (columns of one matrix) are refused too, clip what they are views of.
+    Gradients that were computed with create_graph=True are scaled as plain values."""
     max_norm = _checked_max_norm(max_norm)
     gl = _GradList(grads, True)
     if gl.device is None:

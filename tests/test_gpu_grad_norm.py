@@ -465,3 +465,16 @@ def test_traces_and_forward_mode_are_refused():
     assert torch.equal(g, torch.tensor([3.0, 4.0], device="cuda"))
     with fw.dual_level():
         assert float(A.grad_norm([g])) == 5.0                                    # a level that is open, no tangent
+
+
+def test_interleaved_views_are_refused_by_name_and_their_base_is_taken():
+    m = torch.arange(64.0, device="cuda").view(8, 8)
+    keep = m.clone()
+    views = [m[:, :4], m[:, 4:]]
+    with pytest.raises(ValueError, match="interleave"):
+        A.clip_grad_norm_(views, 1.0)
+    assert torch.equal(m, keep)
+    same_norm(A.grad_norm(views), [keep])                                        # reading them is fine
+    same_norm(A.clip_grad_norm_(m, 1.0), [keep])
+    A.clip_grad_norm_([keep[:4], keep[4:]], 1.0)                                 # as are views that lie one behind the other
+    assert torch.equal(m, keep)
