@@ -351,6 +351,8 @@ class GraphAdam:
 
     def _clipped_step(self, L, numel, cols, tick: bool, gp, stream) -> None:
         n = len(numel)
+        if len(set(cols[0])) != n:                 # the workgroups of both entries would update the same elements at once
+            raise ValueError("GraphAdam: a parameter is listed twice (tied weights?): list it once")
         addresses = [(C.c_void_p * n)(*c) for c in cols]
         with on_device(self.device):
             # the partial sums of this step: allocated per step, so that two captured steps never share them

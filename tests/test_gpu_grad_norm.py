@@ -478,3 +478,15 @@ def test_interleaved_views_are_refused_by_name_and_their_base_is_taken():
     same_norm(A.clip_grad_norm_(m, 1.0), [keep])
     A.clip_grad_norm_([keep[:4], keep[4:]], 1.0)                                 # as are views that lie one behind the other
     assert torch.equal(m, keep)
+
+
+def test_a_parameter_listed_twice_is_refused():
+    p, q = (torch.nn.Parameter(torch.ones(n, device="cuda")) for n in (5000, 3))
+    for groups in ([p, q, p], [{"params": [p]}, {"params": [q, p]}], [p, q, torch.nn.Parameter(p.detach())]):
+        opt = A.GraphAdam(groups, lr=1e-2, max_norm=1.0)
+        for g in opt.param_groups:
+            for t in g["params"]:
+                t.grad = torch.ones_like(t)
+        with pytest.raises(ValueError, match="listed twice"):
+            opt.step()
+        assert torch.equal(p, torch.ones_like(p)) and opt.step_count == 0
