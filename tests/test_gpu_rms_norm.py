@@ -98,6 +98,25 @@ def test_against_64_bits(shape, dtype, residual):
     check(shape, dtype, [None, "same", "float32"][(sum(shape) + residual) % 3], residual)
 
 
+# What the sizes above do not reach of the map kernels: 64 floats of a channel a workgroup (at least 32768 pixels), loads past the
+# caches (128 MiB and more), several tiles a workgroup of several waves (its share of dweight, and the two LDS buffers by turns),
+# one pixel a vector with more than one channel, the border between two forms.
+@pytest.mark.parametrize("shape,dtype", [
+    ((2, 128, 256, 256), torch.float32), ((1, 256, 181, 182), torch.float32), ((1, 30, 181, 182), torch.float32),
+    ((3, 250, 96, 116), torch.float32), ((4, 100, 90, 91), torch.bfloat16), ((2, 512, 128, 128), torch.bfloat16), ((1, 300, 330, 331), torch.float16), ((1, 200, 590, 591), torch.bfloat16),
+    ((1, 32, 1024, 1024), torch.float16), ((2, 520, 180, 180), torch.bfloat16), ((1, 1000, 257, 255), torch.bfloat16), ((9, 600, 61, 64), torch.float32)], ids=str)
+@pytest.mark.parametrize("residual", [False, True], ids=["plain", "residual"])
+def test_large_maps(shape, dtype, residual):
+    check(shape, dtype, "float32", residual, seed=3)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("C", [5, 300, 600, 1024])
+@pytest.mark.parametrize("pixels", [(3, 2, 1), (2, 1, 7), (2, 3, 1), (400, 1, 3)], ids=str)
+def test_maps_narrower_than_a_vector(pixels, C, dtype):
+    check((pixels[0], C, pixels[1], pixels[2]), dtype, ["same", "float32", None][C % 3], C != 300, seed=4)
+
+
 @pytest.mark.parametrize("weight", [None, "same", "float32"], ids=str)
 @pytest.mark.parametrize("shape", [(129, 770), (2, 40, 30, 31)], ids=str)
 def test_weights(shape, weight):
