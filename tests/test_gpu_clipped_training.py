@@ -42,6 +42,46 @@ def test_network_with_norm_against_its_native_twin():
         assert _rel(outs[0][1][n], outs[1][1][n]) <= 1e-6, n
 
 
+def test_network_with_norm_in_half_precision(monkeypatch):
+    """The 16-bit network, forward and backward: every rms_norm call that it makes against its definition in 64 bits, and the gains'
+    gradients.  (The convolutions, not this library's, are computed in float and rounded.)"""
+    from test_gpu_rms_norm import held, reference
+    for name in ("conv2d", "conv_transpose2d"):
+        def wide(x, w, b=None, fn=getattr(SN.F, name), **kw):
+            return fn(x.float(), w.float(), None if b is None else b.float(), **kw).to(x.dtype)
+        monkeypatch.setattr(SN.F, name, wide)
+    calls, plain = [], SN.rms_norm
+
+    def recorded(x, weight=None, residual=None, **kw):
+        out = plain(x, weight, residual=residual, **kw)
+        y = out if residual is None else out[0]
+        call = {"in": [None if t is None else t.detach() for t in (x, weight, residual)], "y": y.detach()}
+        if y.requires_grad:
+            y.register_hook(lambda g: call.__setitem__("gy", g.detach()))
+        calls.append(call)
+        return out
+    monkeypatch.setattr(SN, "rms_norm", recorded)
+    torch.manual_seed(5)
+    net = SN.StyleUNetLite(size=64, out_ch=7, style_dim=32, channels={k: min(v, 24) for k, v in SN.CHANNELS.items()}, norm="rms").cuda().half()
+    with torch.no_grad():
+        for p in net.gains:
+            p.uniform_(0.5, 1.5)
+    g = torch.Generator().manual_seed(6)
+    cond, style = torch.randn(2, 4, 64, 64, generator=g).cuda().half(), torch.randn(2, 32, generator=g).cuda().half()
+    out = net(cond, style)
+    (out.float() * torch.randn(2, 7, 64, 64, generator=g).cuda()).sum().backward()
+    assert out.dtype is torch.float16 and torch.isfinite(out).all() and len(calls) == 1 + len(net.gains)
+    for call, gain in zip(calls, [None, *net.gains]):
+        x, w, r = call["in"]
+        assert x.dtype is torch.float16 and (r is None) == (gain is None)
+        gy = call.get("gy", torch.zeros_like(x))
+        ref, size = reference(x, w, r, gy, None, eps=1e-8)
+        held("y", call["y"], ref["y"], size["y"], x.shape[1], 1, torch.float16)
+        if gain is not None:
+            assert "gy" in call and gy.any()
+            held("dw", gain.grad, ref["dw"], size["dw"], x.shape[1], x.numel() // x.shape[1], torch.float16)
+
+
 def test_captured_appearance_iteration_with_norm_and_clipping():
     """Replays of the captured iteration (network with rms_norm, clipped update) against the same iteration run eagerly."""
     from ggsplat.inner_step import DEFAULT_OPT, GraphedAppearanceStep, appearance_step
