@@ -767,8 +767,15 @@ template <typename T, bool SECOND> void launch_dw(const NormArgs<T>& a, hipStrea
     else hipLaunchKernelGGL((k_rms_dw<T, true, SECOND>), dim3(a.C, a.n_partial), dim3(256), 0, s, a);
 }
 
+// dw from a.n_partial rows of partials (none at all: zeros)
+template <typename T> int sum_dw(const char* who, const NormArgs<T>& a, hipStream_t s) {
+    hipLaunchKernelGGL((k_rms_dw_sum<T>), dim3((a.C + 7) / 8), dim3(1024), 0, s, a);
+    return launched(who);
+}
+
 template <typename T> int run_backward(NormArgs<T> a, hipStream_t s) {
     const char* who = "ggs_rms_norm_backward";
+    if (a.outer == 0 || a.inner == 0) return a.dw ? sum_dw(who, a, s) : GGS_OK;
     const Plan p = plan<T>(a.outer, a.C, a.inner);
     if (p.kind) {
         one_pass(true, a, p, s);
@@ -781,13 +788,12 @@ template <typename T> int run_backward(NormArgs<T> a, hipStream_t s) {
     a.n_partial = p.partials;
     if (!p.kind) launch_dw<T, false>(a, s);
     rc = launched(who);
-    if (rc != GGS_OK) return rc;
-    hipLaunchKernelGGL((k_rms_dw_sum<T>), dim3((a.C + 7) / 8), dim3(1024), 0, s, a);
-    return launched(who);
+    return rc != GGS_OK ? rc : sum_dw(who, a, s);
 }
 
 template <typename T> int run_second(NormArgs<T> a, hipStream_t s) {
     const char* who = "ggs_rms_norm_double_backward";
+    if (a.outer == 0 || a.inner == 0) return a.dw ? sum_dw(who, a, s) : GGS_OK;
     if (a.inner == 1) hipLaunchKernelGGL((k_rms_second<T, false>), dim3(two_pass_blocks(a)), dim3(1024), 0, s, a);
     else hipLaunchKernelGGL((k_rms_second<T, true>), dim3(two_pass_blocks(a)), dim3(1024), 0, s, a);
     int rc = launched(who);
@@ -795,9 +801,7 @@ template <typename T> int run_second(NormArgs<T> a, hipStream_t s) {
     a.n_partial = two_pass_partials(a.outer, a.inner);
     launch_dw<T, true>(a, s);
     rc = launched(who);
-    if (rc != GGS_OK) return rc;
-    hipLaunchKernelGGL((k_rms_dw_sum<T>), dim3((a.C + 7) / 8), dim3(1024), 0, s, a);
-    return launched(who);
+    return rc != GGS_OK ? rc : sum_dw(who, a, s);
 }
 
 size_t partials(int dtype, size_t outer, int C, size_t inner) {
@@ -892,9 +896,9 @@ int ggs_rms_norm_backward(int dtype, size_t outer, int channels, size_t inner, c
     ggs_clear_error_();
     int rc = check_sizes("ggs_rms_norm_backward", dtype, outer, channels, inner, 1.0);
     if (rc != GGS_OK) return rc;
-    if (outer == 0 || inner == 0) return GGS_OK;
-    if (!x || !q || !gy || !dx) return ggs_fail_(GGS_ERR_ARG, "ggs_rms_norm_backward: NULL pointer argument");
-    if (dw && (!workspace || workspace_bytes < ggs_rms_norm_workspace_bytes(dtype, outer, channels, inner)))
+    if (outer && inner && (!x || !q || !gy || !dx)) return ggs_fail_(GGS_ERR_ARG, "ggs_rms_norm_backward: NULL pointer argument");
+    const size_t needed = dw ? ggs_rms_norm_workspace_bytes(dtype, outer, channels, inner) : 0;
+    if (needed && (!workspace || workspace_bytes < needed))
         return ggs_fail_(GGS_ERR_SIZE, "ggs_rms_norm_backward: the workspace is too small (ggs_rms_norm_workspace_bytes)");
     hipStream_t s = (hipStream_t)stream;
     switch (dtype) {
@@ -915,9 +919,8 @@ int ggs_rms_norm_double_backward(int dtype, size_t outer, int channels, size_t i
     ggs_clear_error_();
     int rc = check_sizes("ggs_rms_norm_double_backward", dtype, outer, channels, inner, 1.0);
     if (rc != GGS_OK) return rc;
-    if (outer == 0 || inner == 0) return GGS_OK;
-    if (!x || !q || !gy || !dh || !dgy) return ggs_fail_(GGS_ERR_ARG, "ggs_rms_norm_double_backward: NULL pointer argument");
-    if (!workspace || workspace_bytes < second_bytes(dtype, outer, channels, inner))
+    if (outer && inner && (!x || !q || !gy || !dh || !dgy)) return ggs_fail_(GGS_ERR_ARG, "ggs_rms_norm_double_backward: NULL pointer argument");
+    if (outer && inner && (!workspace || workspace_bytes < second_bytes(dtype, outer, channels, inner)))
         return ggs_fail_(GGS_ERR_SIZE, "ggs_rms_norm_double_backward: the workspace is too small (ggs_rms_norm_double_workspace_bytes)");
     hipStream_t s = (hipStream_t)stream;
     switch (dtype) {

@@ -264,11 +264,8 @@ def _rms_backward(x, residual, w, q, gy, gh, plan, need_dw):
         if need_dw:
             dw = torch.empty_like(w)
             nb = _rms_workspace_bytes(code, outer, c, inner)
-            if nb:
-                ws = q.new_empty(nb // q.element_size())              # (the accumulation type, as q)
-                dwp, wp = dw.data_ptr(), ws.data_ptr()
-            else:
-                dw.zero_()                                            # no pixels
+            ws = q.new_empty(nb // q.element_size())                  # (the accumulation type, as q)
+            dwp, wp = dw.data_ptr(), ws.data_ptr()
         rc = L.ggs_rms_norm_backward(code, outer, c, inner, x.data_ptr(), None if residual is None else residual.data_ptr(),
                                      None if w is None else w.data_ptr(), w32, q.data_ptr(), gy.data_ptr(), gp, dx.data_ptr(), dwp, wp,
                                      nb, stream_ptr(dev))
@@ -304,8 +301,6 @@ class _RmsNormGrad(torch.autograd.Function):
         with on_device(dev):
             nb = L.ggs_rms_norm_double_workspace_bytes(code, outer, c, inner)
             ws = torch.empty(nb, dtype=torch.uint8, device=dev)
-            if dw is not None and nb == 0:
-                dw.zero_()                                            # no pixels
             check(L.ggs_rms_norm_double_backward(code, outer, c, inner, x.data_ptr(), None if residual is None else residual.data_ptr(),
                                                  ptr(w), w32, q.data_ptr(), gy.data_ptr(), None if v is None else v.data_ptr(), ptr(u),
                                                  dh.data_ptr(), dgy.data_ptr(), ptr(dw), ws.data_ptr(), nb, stream_ptr(dev)),

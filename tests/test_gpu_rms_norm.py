@@ -454,3 +454,21 @@ def test_traced_calls():
         dx, dr, dw = torch.autograd.grad((y, h), leaves, (gy, gh))
         for k, v in (("y", y), ("h", h), ("dx", dx), ("dr", dr), ("dw", dw)):
             assert torch.equal(v, want[k]), k
+
+
+@pytest.mark.parametrize("weight_f32", [0, 1])
+@pytest.mark.parametrize("code,dtype", [(0, torch.float32), (1, torch.float16), (2, torch.float64), (3, torch.bfloat16)])
+def test_no_pixels_give_a_dweight_of_zeros(code, dtype, weight_f32):
+    """The C entry points: with no pixel there is nothing to read and no workspace, and dw is a sum of nothing."""
+    L, C = _lib.lib(), 301
+    s = torch.cuda.current_stream().cuda_stream
+    for outer, inner in ((0, 1), (0, 7), (3, 0)):
+        assert L.ggs_rms_norm_workspace_bytes(code, outer, C, inner) == L.ggs_rms_norm_double_workspace_bytes(code, outer, C, inner) == 0
+        for double in (False, True):
+            buf = torch.full((C + 64,), 7.0, device="cuda", dtype=torch.float32 if weight_f32 else dtype)
+            dw = buf[32:32 + C].data_ptr()
+            if double:
+                rc = L.ggs_rms_norm_double_backward(code, outer, C, inner, None, None, None, weight_f32, None, None, None, None, None, None, dw, None, 0, s)
+            else:
+                rc = L.ggs_rms_norm_backward(code, outer, C, inner, None, None, None, weight_f32, None, None, None, None, dw, None, 0, s)
+            assert rc == 0 and not buf[32:32 + C].any() and (buf[:32] == 7).all() and (buf[32 + C:] == 7).all()
