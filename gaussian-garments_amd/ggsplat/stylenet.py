@@ -324,7 +324,8 @@ def rms_norm(x, weight=None, residual=None, eps: float = 1e-8, impl: str = "hip"
     """y = weight[channel] * h / sqrt(mean over the channels of h^2 + eps), h = x (+ residual), for x [B, C, ...] (every pixel of a
     feature map by itself; [rows, C]: every row).  Returns y, or (y, h) with a residual -- h is the sum to carry on.
     x, residual: float32 / float16 / bfloat16 / float64, the same shape; weight [C]: x's type or float32; contiguous and
-    channels-last maps are taken as they are.  The norm is that of the unrounded sum; sums are in float (double for float64).
+    channels-last maps are taken as they are.  The norm is that of the unrounded sum; sums are in float (double for float64), so the
+    squares of a pixel have to stay below 3.4e38 in all (y is 0 beyond) and eps counts as at least 1.2e-38 (2.3e-308).
     Differentiable twice (second derivatives are not differentiable again), not in forward mode; torch.jit.trace records a call."""
     _rms_check(x, weight, residual)
     eps = float(eps)

@@ -315,6 +315,8 @@ int ggs_upfirdn2d(int major, int in_h, int in_w, int minor, const float* input, 
  *             computed); that to gh is v.
  * dtype GGS_DTYPE_*: the type of x, residual, y, h, gy, gh, dx, v, dh, dgy.  weight (NULL: 1), u and dw have that type too, or
  * float where weight_f32 != 0.  Sums in float (double for GGS_DTYPE_F64), in an order that does not depend on scheduling.
+ * Range (float sums): h^2 summed over the channels has to stay below 3.4e38, beyond it y is 0 as in plain float arithmetic; eps
+ * counts as at least 1.2e-38 (double: 2.3e-308), so that a pixel of zeros gives zeros.
  * No pixels (outer or inner 0): nothing is read, dw is set to zeros.
  * At most 2^22 channels; tensors need no alignment beyond their element's; outputs overlap neither inputs nor each other.
  * workspace (backward: needed with dw): ggs_rms_norm_workspace_bytes / _double_workspace_bytes(...) bytes, 8-byte aligned, any
