@@ -387,7 +387,9 @@ __global__ __launch_bounds__(1024) void k_planes_forward(NormArgs<T> a) {
 template <typename T, int VEC, int LP, int K, bool NT>
 __global__ __launch_bounds__(1024) void k_planes_backward(NormArgs<T> a, unsigned tiles) {
     __shared__ float lds[2][16 * LP * VEC];
-    constexpr bool EARLY = K * VEC <= 16;    // gh on its way with the rest; where that would spill registers, after the sums
+    // gh on its way with the rest, or after the sums where its registers are not there.  (16 bits with four channels a thread, the
+    // blocks of 257 - 1024 channels, spill 3 - 5 of 128 registers even so: 2 x 512 x 128 x 128 bf16 44 us, 34 at the copy rate.)
+    constexpr bool EARLY = K * VEC <= 16;
     float dw[K] = {}, w[K];
     int turn = 0;
     PlaneTile<VEC, LP>::weights(a, w);
@@ -617,7 +619,7 @@ __global__ __launch_bounds__(1024) void k_rows_backward(NormArgs<T> a, unsigned 
 
 // ---- which kernel ----------------------------------------------------------------------------------------------------------
 // One-pass kernels: float and 16-bit types, a pixel's channels within the registers of one workgroup (1024 channels of a map,
-// 16384 of a row), a map within 32-bit offsets; the two-pass kernels serve double and what is left.
+// 16384 of a row), a map and its q within 32-bit offsets; the two-pass kernels serve double and what is left.
 struct Plan {
     int kind;                    // 0 two passes, 1 planes, 2 rows
     int vec, lanes, k, waves;    // planes: LP and waves of a workgroup; rows: G
